@@ -459,6 +459,44 @@ int sft_leb128_encode(const void *values, int32_t elem_bytes, int64_t n, uint8_t
 int sft_quantize_i16(const float *x, int64_t n, float scale, int16_t *out, void *stream);
 
 /*
+ * ---- Dense head: linear layers ----
+ * y = residual + act(x w^T + bias): the products behind the feature transformer
+ * (the reference's dense layers, src/model/modules/layer_stacks.py,
+ * stacked_linear.py and moe_stacks.py, run on torch's).
+ *   x:        [M, K], rows ldx elements apart; w: [N, K], rows ldw apart
+ *   bias:     [N] or NULL; residual: [M, N], rows ldr apart, or NULL
+ *   y:        [M, N], rows ldy apart (may be residual itself)
+ *   deriv:    dense [M, N], or NULL: act' at every output, for sft_linear_bwd;
+ *             float for SFT_TYPE_F32, else int16 fixed point with 14 fractional bits.
+ *             Not used for SFT_ACT_NONE.
+ * All tensors but deriv have the type `dtype`; sums are binary32, y is rounded once.
+ * The backward reads dy ([M, N], rows lddy apart) and the forward's deriv and writes
+ * dense dx [M, K], dw [N, K] and db [N], each NULL if not wanted (the residual's
+ * gradient is dy).  Results do not vary from run to run.
+ * K and N in [1, 2^26], M in [0, 2^30]; M = 0 is no rows: an empty y, zero dw and db.
+ */
+#define SFT_TYPE_F32 0
+#define SFT_TYPE_F16 1
+#define SFT_TYPE_BF16 2
+#define SFT_ACT_NONE 0
+#define SFT_ACT_RELU 1   /* max(z, 0)                  */
+#define SFT_ACT_CRELU 2  /* clamp(z, 0, 1)             */
+#define SFT_ACT_SCRELU 3 /* clamp(z, 0, 1)^2           */
+#define SFT_ACT_SILU 4   /* z / (1 + exp(-z))          */
+#define SFT_ACT_GELU 5   /* z Phi(z), the exact form   */
+int sft_linear_fwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, size_t *bytes);
+int sft_linear_fwd(int32_t dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,
+                   const void *bias, const void *residual, int64_t ldr, void *y, int64_t ldy,
+                   void *deriv, int64_t M, int64_t K, int64_t N, int32_t act, void *workspace,
+                   size_t workspace_bytes, void *stream);
+int sft_linear_bwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, int32_t act,
+                                  size_t *bytes);
+int sft_linear_bwd(int32_t dtype, const void *dy, int64_t lddy, const void *deriv, const void *x,
+                   int64_t ldx, const void *w, int64_t ldw, void *dx, void *dw, void *db, int64_t M,
+                   int64_t K, int64_t N, int32_t act, void *workspace, size_t workspace_bytes,
+                   void *stream);
+
+/*
  * Measurement helper (no reference counterpart): one dispatch of `blocks`
  * 256-thread workgroups whose 8-lane groups each gather 8 * rounds 128-byte rows
  * of table (table_rows x 128 bytes, table_rows a power of two <= 2^24, 16-byte

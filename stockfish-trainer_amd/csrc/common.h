@@ -84,6 +84,8 @@ enum ProfKind : int {
   kProfLeb128,
   kProfProbeL2Gather,
   kProfFwdRanks,
+  kProfDenseProduct,
+  kProfDenseActBwd,
   kProfNumKinds
 };
 struct ProfScope {

@@ -35,6 +35,15 @@ SFT_BWD_PREPARED = 0x20
 SFT_Q16_ACC32 = 0x0
 SFT_Q16_WRAP16 = 0x1
 SFT_Q16_ROWS = 0x2
+SFT_TYPE_F32 = 0
+SFT_TYPE_F16 = 1
+SFT_TYPE_BF16 = 2
+SFT_ACT_NONE = 0
+SFT_ACT_RELU = 1
+SFT_ACT_CRELU = 2
+SFT_ACT_SCRELU = 3
+SFT_ACT_SILU = 4
+SFT_ACT_GELU = 5
 SFT_FEATURES_THREATS = 1
 SFT_FEATURES_HALFKA = 2
 
@@ -113,6 +122,17 @@ SIGNATURES = {
     "sft_leb128_workspace_size": (ctypes.c_int, [_i64, ctypes.POINTER(ctypes.c_size_t)]),
     "sft_leb128_encode": (ctypes.c_int, [_vp, _i32, _i64, _vp, ctypes.c_size_t, _vp, _vp, ctypes.c_size_t, _vp]),
     "sft_quantize_i16": (ctypes.c_int, [_vp, _i64, ctypes.c_float, _vp, _vp]),
+    "sft_linear_fwd_workspace_size": (ctypes.c_int, [_i32, _i64, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)]),
+    "sft_linear_fwd": (
+        ctypes.c_int,
+        [_i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, ctypes.c_size_t,
+         _vp]),
+    "sft_linear_bwd_workspace_size": (
+        ctypes.c_int, [_i32, _i64, _i64, _i64, _i32, ctypes.POINTER(ctypes.c_size_t)]),
+    "sft_linear_bwd": (
+        ctypes.c_int,
+        [_i32, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, ctypes.c_size_t,
+         _vp]),
     "sft_probe_l2_gather": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
     "sft_prof_enable": (ctypes.c_int, [ctypes.c_int]),
     "sft_prof_num_kinds": (ctypes.c_int, []),
@@ -741,6 +761,61 @@ def quantize_i16(x: torch.Tensor, scale: float) -> torch.Tensor:
         _check(lib().sft_quantize_i16(_ptr(x), x.numel(), float(scale), _ptr(out), _stream(x.device)),
                "sft_quantize_i16")
     return out
+
+
+# ---- the dense head ----
+_TYPES = {torch.float32: SFT_TYPE_F32, torch.float16: SFT_TYPE_F16, torch.bfloat16: SFT_TYPE_BF16}
+
+
+def type_code(dtype: torch.dtype) -> int:
+    code = _TYPES.get(dtype)
+    _require(code is not None, f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    return code
+
+
+def _rows(t: torch.Tensor):
+    """Row stride of a 2-D tensor whose rows are dense (a tensor of one row or column has any)."""
+    rows, cols = t.shape
+    _require(cols == 1 or t.stride(1) == 1, "rows must be dense (stride 1 in the last dimension)")
+    return t.stride(0) if rows > 1 and t.stride(0) >= cols else cols
+
+
+def _scratch(nbytes: int, device: torch.device):
+    """(keep-alive tensor or None, pointer) of a device workspace; torch's allocator aligns to 512 bytes."""
+    if nbytes == 0:
+        return None, None
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return buf, buf.data_ptr()
+
+
+def linear_fwd(x, w, bias, residual, y, deriv, act: int) -> None:
+    """y = residual + act(x w^T + bias) of 2-D tensors with dense rows; deriv (or None) gets act'."""
+    (M, K), N = x.shape, w.shape[0]
+    code = type_code(x.dtype)
+    dev = x.device
+    n = ctypes.c_size_t(0)
+    _check(lib().sft_linear_fwd_workspace_size(code, M, K, N, ctypes.byref(n)), "sft_linear_fwd_workspace_size")
+    with torch.cuda.device(dev):
+        keep, ws = _scratch(n.value, dev)
+        _check(lib().sft_linear_fwd(code, _ptr(x), _rows(x), _ptr(w), _rows(w), _ptr(bias), _ptr(residual),
+                                    0 if residual is None else _rows(residual), _ptr(y), _rows(y), _ptr(deriv), M, K,
+                                    N, act, ws, n.value, _stream(dev)), "sft_linear_fwd")
+    del keep
+
+
+def linear_bwd(dy, deriv, x, w, dx, dw, db, act: int) -> None:
+    """dx, dw and db (each may be None) of linear_fwd's y from dy and its deriv."""
+    (M, K), N = x.shape, w.shape[0]
+    code = type_code(dy.dtype)
+    dev = dy.device
+    n = ctypes.c_size_t(0)
+    _check(lib().sft_linear_bwd_workspace_size(code, M, K, N, act, ctypes.byref(n)), "sft_linear_bwd_workspace_size")
+    with torch.cuda.device(dev):
+        keep, ws = _scratch(n.value, dev)
+        _check(lib().sft_linear_bwd(code, _ptr(dy), _rows(dy), _ptr(deriv), _ptr(x), _rows(x), _ptr(w), _rows(w),
+                                    _ptr(dx), _ptr(dw), _ptr(db), M, K, N, act, ws, n.value, _stream(dev)),
+               "sft_linear_bwd")
+    del keep
 
 
 # ---- per-launch kernel timing ----
