@@ -497,6 +497,49 @@ int sft_linear_bwd(int32_t dtype, const void *dy, int64_t lddy, const void *deri
                    void *stream);
 
 /*
+ * ---- Dense head: the router's balance loss ----
+ * (for routers such as the reference's, src/model/modules/moe_stacks.py)
+ *   logits: [rows, experts], rows ld elements apart; mask: uint8 [rows], 0 leaves
+ *   the position out, or NULL
+ *   p = softmax(logits) per position; its top_k experts are chosen by logit, equal
+ *   ones by the lower number, never one at -inf
+ *   counts[e] = positions that chose e; *kept = n, the positions that count: not
+ *   masked, and with a logit above -inf
+ *   *loss = experts * sum_e (counts[e] / (n top_k)) (sum of p_e / n); 0 if n = 0
+ * The backward writes dense grad_logits [rows, experts] = *grad_loss times the
+ * loss's gradient, the counts held constant; zeros for positions left out, whatever
+ * they hold.  loss and grad_loss are float, counts and kept int64, all on the
+ * device.  Results do not vary from run to run.
+ */
+#define SFT_BALANCE_MAX_EXPERTS 1024
+int sft_balance_fwd_workspace_size(int32_t dtype, int64_t rows, int32_t experts, size_t *bytes);
+int sft_balance_fwd(int32_t dtype, const void *logits, int64_t ld, const uint8_t *mask,
+                    int64_t rows, int32_t experts, int32_t top_k, float *loss, int64_t *counts,
+                    int64_t *kept, void *workspace, size_t workspace_bytes, void *stream);
+int sft_balance_bwd(int32_t dtype, const void *logits, int64_t ld, const uint8_t *mask,
+                    int64_t rows, int32_t experts, int32_t top_k, const int64_t *counts,
+                    const int64_t *kept, const float *grad_loss, void *grad_logits, void *stream);
+
+/*
+ * ---- Dense head: distillation from a teacher's top classes ----
+ * (no reference counterpart; for heads that predict moves)
+ *   student: [rows, classes], rows lds elements apart; teacher: dense [rows, k] logits
+ *   of the classes in indices (dense int32 or int64 [rows, k]; an index outside
+ *   [0, classes) leaves its slot empty)
+ *   p = softmax(student / T), q = softmax(teacher / T) over the filled slots
+ *   loss[row] = T^2 sum_j q_j (log q_j - log p_{i_j})
+ *   grad_student[row] = row_weight[row] (1 if NULL) T (p - q): dense [rows, classes]
+ * Either output may be NULL.  Slots with q = 0 add nothing.  A row without a filled
+ * slot above -inf, or without a class above -inf, has loss 0 and gradient 0.
+ * row_weight and loss are float.
+ */
+#define SFT_DISTILL_MAX_K 256
+int sft_distill(int32_t dtype, const void *student, int64_t lds, int32_t teacher_dtype,
+                const void *teacher, const void *indices, int32_t index_bytes, int64_t rows,
+                int64_t classes, int32_t k, float temperature, const float *row_weight,
+                float *loss, void *grad_student, void *stream);
+
+/*
  * Measurement helper (no reference counterpart): one dispatch of `blocks`
  * 256-thread workgroups whose 8-lane groups each gather 8 * rounds 128-byte rows
  * of table (table_rows x 128 bytes, table_rows a power of two <= 2^24, 16-byte

@@ -2,6 +2,7 @@
 // reporting and the optional per-launch event timing.
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <initializer_list>
 #include <memory>
 #include <mutex>
@@ -70,6 +71,13 @@ size_t linear_bwd_workspace(int dtype, int64_t M, int64_t K, int64_t N, int act)
 int linear_bwd(int dtype, const void *dy, int64_t lddy, const void *deriv, const void *x, int64_t ldx, const void *w,
                int64_t ldw, void *dx, void *dw, void *db, int64_t M, int64_t K, int64_t N, int act, void *ws,
                hipStream_t s);
+size_t balance_fwd_workspace(int dtype, int64_t rows, int E);
+int balance_fwd(int dtype, const void *logits, int64_t ld, const uint8_t *mask, int64_t rows, int E, int top_k,
+                float *loss, int64_t *counts, int64_t *kept, void *ws, hipStream_t s);
+int balance_bwd(int dtype, const void *logits, int64_t ld, const uint8_t *mask, int64_t rows, int E, int top_k,
+                const int64_t *counts, const int64_t *kept, const float *grad, void *out, hipStream_t s);
+int distill(int dtype, const void *student, int64_t lds, int ttype, const void *teacher, const void *idx, int idx64,
+            int64_t rows, int V, int k, float tau, const float *weight, float *loss, void *ds, hipStream_t s);
 size_t map_tiles_workspace(const ColMap &m, int64_t rows);
 size_t table_tiles_workspace(const ColMap &m, int64_t N);
 size_t fwd_pair_workspace(const ColMap &m, int64_t B, int K, int64_t N, bool carry);
@@ -257,6 +265,7 @@ const char *const kKindNames[] = {
     "fwd_tile_relayout", "fwd_f32_tiled_gather", "bwd_tiled_gather", "fwd_i16_tiled_gather",
     "fwd_fold_relayout", "bwd_virtual_reduce", "bwd_epilogue", "ranger22_update", "encode_features", "leb128_encode",
     "probe_l2_gather", "fwd_rank_lists", "dense_product", "dense_act_bwd",
+    "dense_balance", "dense_distill",
 };
 static_assert(sizeof(kKindNames) / sizeof(kKindNames[0]) == kProfNumKinds, "one name per profiling kind");
 }  // namespace
@@ -312,6 +321,17 @@ bool misaligned(int32_t dtype, std::initializer_list<const void *> ptrs) {
   for (const void *p : ptrs)
     if ((uintptr_t)p % size) return true;
   return false;
+}
+
+// A router's sizes and type.
+bool bad_balance(int32_t dtype, int64_t rows, int32_t experts, int32_t top_k, int64_t ld, std::string &why) {
+  if (dtype < SFT_TYPE_F32 || dtype > SFT_TYPE_BF16) why = "unknown type";
+  else if (rows < 0 || rows > ((int64_t)1 << 30)) why = "rows must be in [0, 2^30]";
+  else if (experts < 1 || experts > SFT_BALANCE_MAX_EXPERTS) why = "experts must be in [1, SFT_BALANCE_MAX_EXPERTS]";
+  else if (top_k < 1 || top_k > experts) why = "top_k must be in [1, experts]";
+  else if (bad_stride(ld, experts)) why = "the row stride is smaller than a row, or 2^40 or more";
+  else return false;
+  return true;
 }
 
 // The forward's flags: at most one of rows and tiles.
@@ -849,6 +869,74 @@ int sft_linear_bwd(int32_t dtype, const void *dy, int64_t lddy, const void *deri
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256))
     return fail(SFT_EWORKSPACE, std::string(who) + ": needs " + std::to_string(need) + " bytes, 256-byte aligned");
   return linear_bwd(dtype, dy, lddy, deriv, x, ldx, w, ldw, dx, dw, db, M, K, N, act, workspace, (hipStream_t)stream);
+}
+
+int sft_balance_fwd_workspace_size(int32_t dtype, int64_t rows, int32_t experts, size_t *bytes) {
+  clear_error();
+  const char *who = "sft_balance_fwd_workspace_size";
+  std::string why;
+  if (!bytes) return fail(SFT_EINVAL, std::string(who) + ": null pointer");
+  if (bad_balance(dtype, rows, experts, 1, experts, why)) return fail(SFT_EINVAL, std::string(who) + ": " + why);
+  *bytes = balance_fwd_workspace(dtype, rows, experts);
+  return SFT_OK;
+}
+
+int sft_balance_fwd(int32_t dtype, const void *logits, int64_t ld, const uint8_t *mask, int64_t rows, int32_t experts,
+                    int32_t top_k, float *loss, int64_t *counts, int64_t *kept, void *workspace,
+                    size_t workspace_bytes, void *stream) {
+  clear_error();
+  const char *who = "sft_balance_fwd";
+  std::string why;
+  if (bad_balance(dtype, rows, experts, top_k, ld, why)) return fail(SFT_EINVAL, std::string(who) + ": " + why);
+  if ((rows > 0 && !logits) || !loss || !counts || !kept) return fail(SFT_EINVAL, std::string(who) + ": null pointer");
+  if (misaligned(dtype, {logits}) || (uintptr_t)loss % 4 || ((uintptr_t)counts | (uintptr_t)kept) % 8)
+    return fail(SFT_EINVAL, std::string(who) + ": a tensor is not aligned to its type");
+  const size_t need = balance_fwd_workspace(dtype, rows, experts);
+  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)
+    return fail(SFT_EWORKSPACE, std::string(who) + ": needs " + std::to_string(need) + " bytes, 256-byte aligned");
+  return balance_fwd(dtype, logits, ld, mask, rows, experts, top_k, loss, counts, kept, workspace,
+                     (hipStream_t)stream);
+}
+
+int sft_balance_bwd(int32_t dtype, const void *logits, int64_t ld, const uint8_t *mask, int64_t rows, int32_t experts,
+                    int32_t top_k, const int64_t *counts, const int64_t *kept, const float *grad_loss,
+                    void *grad_logits, void *stream) {
+  clear_error();
+  const char *who = "sft_balance_bwd";
+  std::string why;
+  if (bad_balance(dtype, rows, experts, top_k, ld, why)) return fail(SFT_EINVAL, std::string(who) + ": " + why);
+  if (rows == 0) return SFT_OK;
+  if (!logits || !counts || !kept || !grad_loss || !grad_logits)
+    return fail(SFT_EINVAL, std::string(who) + ": null pointer");
+  if (misaligned(dtype, {logits, grad_logits}) || (uintptr_t)grad_loss % 4 || ((uintptr_t)counts | (uintptr_t)kept) % 8)
+    return fail(SFT_EINVAL, std::string(who) + ": a tensor is not aligned to its type");
+  return balance_bwd(dtype, logits, ld, mask, rows, experts, top_k, counts, kept, grad_loss, grad_logits,
+                     (hipStream_t)stream);
+}
+
+int sft_distill(int32_t dtype, const void *student, int64_t lds, int32_t teacher_dtype, const void *teacher,
+                const void *indices, int32_t index_bytes, int64_t rows, int64_t classes, int32_t k, float temperature,
+                const float *row_weight, float *loss, void *grad_student, void *stream) {
+  clear_error();
+  const char *who = "sft_distill";
+  auto bad = [&](const char *why) { return fail(SFT_EINVAL, std::string(who) + ": " + why); };
+  if (dtype < SFT_TYPE_F32 || dtype > SFT_TYPE_BF16 || teacher_dtype < SFT_TYPE_F32 || teacher_dtype > SFT_TYPE_BF16)
+    return bad("unknown type");
+  if (index_bytes != 4 && index_bytes != 8) return bad("index_bytes must be 4 or 8");
+  if (rows < 0 || rows >= ((int64_t)1 << 30)) return bad("rows must be in [0, 2^30)");
+  if (classes < 1 || classes > ((int64_t)1 << 28)) return bad("classes must be in [1, 2^28]");
+  if (k < 1 || k > SFT_DISTILL_MAX_K) return bad("k must be in [1, SFT_DISTILL_MAX_K]");
+  if (rows * classes >= (1ll << 40)) return bad("tensor too large");
+  if (bad_stride(lds, classes)) return bad("the row stride is smaller than a row, or 2^40 or more");
+  if (!(temperature > 0.f) || !(temperature < INFINITY)) return bad("temperature must be positive and finite");
+  if (rows == 0) return SFT_OK;
+  if (!loss && !grad_student) return bad("neither loss nor grad_student");
+  if (!student || !teacher || !indices) return bad("null pointer");
+  if (misaligned(dtype, {student, grad_student}) || misaligned(teacher_dtype, {teacher}) ||
+      (uintptr_t)indices % index_bytes || ((uintptr_t)row_weight | (uintptr_t)loss) % 4)
+    return bad("a tensor is not aligned to its type");
+  return distill(dtype, student, lds, teacher_dtype, teacher, indices, index_bytes == 8, rows, (int)classes, k,
+                 temperature, row_weight, loss, grad_student, (hipStream_t)stream);
 }
 
 int sft_leb128_workspace_size(int64_t n, size_t *bytes) {

@@ -86,6 +86,8 @@ enum ProfKind : int {
   kProfFwdRanks,
   kProfDenseProduct,
   kProfDenseActBwd,
+  kProfDenseBalance,
+  kProfDenseDistill,
   kProfNumKinds
 };
 struct ProfScope {

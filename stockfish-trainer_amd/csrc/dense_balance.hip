@@ -1,0 +1,382 @@
+// The router's balance loss.  For the kept positions t of n, with p = softmax of a
+// position's logits and S_t its top_k experts:
+//   counts_e = #{t : e in S_t},  f_e = counts_e / (n top_k),  P_e = mean_t p_te
+//   loss     = E sum_e f_e P_e
+//   d loss / d logit_tj = E / n p_tj (f_j - sum_e f_e p_te)      (f is piecewise constant)
+// A position is kept if its mask byte is set (or there is no mask) and some logit is
+// above -inf.  Experts are chosen by logit, equal ones by the lower number; those at
+// -inf are never chosen.
+//
+// Bound by reading the logits (and, in the backward, writing as much): every row is
+// held by a group of G lanes in 16-byte chunks, G the power of two that covers it, so
+// softmax, choice and gradient need one read and shuffles inside the group.  The
+// sums over positions stay in registers of the lane that owns the expert; workgroups
+// write partials that one more launch adds in a fixed order, in binary64.
+#include "dense.h"
+
+namespace sft {
+
+namespace {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+constexpr int kMaxParts = 512;  // workgroups of the forward, two per CU
+
+template <int G>
+__device__ __forceinline__ float group_max(float x) {
+#pragma unroll
+  for (int m = 1; m < G; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
+  return x;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int m = 1; m < G; m <<= 1) x += __shfl_xor(x, m);
+  return x;
+}
+
+// A row's logits: lane t of the group holds the chunks t + G j of V elements.
+// Elements past E are -inf.
+template <typename T, int G, int C>
+struct Row {
+  static constexpr int V = 16 / (int)sizeof(T);
+  float x[C][V];
+  __device__ __forceinline__ void load(const T *row, int E, int t) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int e0 = (t + G * j) * V;
+      T v[V];
+      if (e0 + V <= E) {
+        __builtin_memcpy(v, row + e0, 16);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[j][i] = (float)v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[j][i] = e0 + i < E ? (float)row[e0 + i] : -INFINITY;
+      }
+    }
+  }
+  __device__ __forceinline__ float max() const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) m = fmaxf(m, x[j][i]);
+    return group_max<G>(m);
+  }
+  // p = exp(x - m) / sum, of a row with m > -inf.
+  __device__ __forceinline__ void softmax(float m, float (&p)[C][V]) const {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        p[j][i] = expf(x[j][i] - m);
+        s += p[j][i];
+      }
+    const float r = 1.f / group_sum<G>(s);
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[j][i] *= r;
+  }
+};
+
+// part_p [parts][E] sums of p, part_c [parts][E] counts, part_n [parts] kept rows.
+template <typename T, int G, int C>
+__global__ __launch_bounds__(kBlock) void balance_fwd_kernel(const T *__restrict__ logits, int64_t ld,
+                                                             const uint8_t *__restrict__ mask, int64_t rows, int E,
+                                                             int top_k, float *__restrict__ part_p,
+                                                             int32_t *__restrict__ part_c,
+                                                             int32_t *__restrict__ part_n) {
+  constexpr int V = Row<T, G, C>::V, kRows = kBlock / G;
+  __shared__ float red_p[kWavesPerBlock][G * C * V];
+  __shared__ int32_t red_c[kWavesPerBlock][G * C * V];
+  __shared__ int32_t red_n[kWavesPerBlock];
+  const int lane = lane_id(), t = lane % G, wave = threadIdx.x / kWave;
+  const uint64_t group = (G == kWave ? ~0ull : ((1ull << (G % kWave)) - 1)) << (lane / G * G);
+  float sum[C][V];
+  int32_t cnt[C][V], kept = 0;
+#pragma unroll
+  for (int j = 0; j < C; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      sum[j][i] = 0.f;
+      cnt[j][i] = 0;
+    }
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t r = r0 + threadIdx.x / G;
+    const bool use = r < rows && (!mask || mask[r]);
+    Row<T, G, C> row;
+    row.load(logits + (use ? r : 0) * ld, use ? E : 0, t);
+    const float m = row.max();
+    const bool keep = use && m > -INFINITY;  // the same in all lanes of a group
+    if (keep) {
+      float p[C][V];
+      row.softmax(m, p);
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[j][i] += p[j][i];
+      kept += t == 0;
+    }
+    // The choice: the largest value left, its lowest element, top_k times.  All lanes
+    // of the wave take part in the shuffles.
+    float best = keep ? m : -INFINITY;
+    for (int k = 0; k < top_k; ++k) {
+      if (k > 0) best = keep ? row.max() : -INFINITY;
+      bool open = best > -INFINITY;  // still to be found, in order of the elements
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        int first = V;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i) first = row.x[j][i] == best ? i : first;
+        const uint64_t hits = ballot(open && first < V) & group;
+        if (hits && lane == __builtin_ctzll(hits)) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (i == first) {
+              ++cnt[j][i];
+              row.x[j][i] = -INFINITY;
+            }
+        }
+        open = open && !hits;
+      }
+    }
+  }
+  // Sums over the row groups of the wave, then over the waves.
+#pragma unroll
+  for (int j = 0; j < C; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+      for (int m = G; m < kWave; m <<= 1) {
+        sum[j][i] += __shfl_xor(sum[j][i], m);
+        cnt[j][i] += __shfl_xor(cnt[j][i], m);
+      }
+      if (lane < G) {
+        red_p[wave][(t + G * j) * V + i] = sum[j][i];
+        red_c[wave][(t + G * j) * V + i] = cnt[j][i];
+      }
+    }
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) kept += __shfl_xor(kept, m);
+  if (lane == 0) red_n[wave] = kept;
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kBlock) {
+    part_p[(int64_t)blockIdx.x * E + e] = (red_p[0][e] + red_p[1][e]) + (red_p[2][e] + red_p[3][e]);
+    part_c[(int64_t)blockIdx.x * E + e] = (red_c[0][e] + red_c[1][e]) + (red_c[2][e] + red_c[3][e]);
+  }
+  if (threadIdx.x == 0) part_n[blockIdx.x] = (red_n[0] + red_n[1]) + (red_n[2] + red_n[3]);
+}
+
+// One workgroup: counts, the number of kept rows and the loss from the partials.
+// Threads (slice, expert): a slice adds every kSlices-th partial, the slices are
+// added in order.
+constexpr int kJoin = 1024;
+__global__ __launch_bounds__(kJoin) void balance_join_kernel(const float *__restrict__ part_p,
+                                                             const int32_t *__restrict__ part_c,
+                                                             const int32_t *__restrict__ part_n, int parts, int E,
+                                                             int top_k, float *__restrict__ loss,
+                                                             int64_t *__restrict__ counts,
+                                                             int64_t *__restrict__ kept) {
+  __shared__ double red_p[kJoin];
+  __shared__ int64_t red_c[kJoin];
+  __shared__ double sums[kJoin / kWave];
+  const int tid = threadIdx.x;
+  int width = 1;
+  while (width < E) width <<= 1;  // <= kJoin
+  const int slices = kJoin / width, e = tid % width, slice = tid / width;
+  // kept rows: wave 0 adds the parts
+  int64_t n = 0;
+  for (int i = tid; i < parts; i += kJoin) n += part_n[i];
+  red_c[tid] = n;
+  __syncthreads();
+  for (int d = kJoin / 2; d > 0; d >>= 1) {
+    if (tid < d) red_c[tid] += red_c[tid + d];
+    __syncthreads();
+  }
+  n = red_c[0];
+  __syncthreads();
+  double p = 0.0;
+  int64_t c = 0;
+  if (e < E)
+    for (int i = slice; i < parts; i += slices) {
+      p += (double)part_p[(int64_t)i * E + e];
+      c += part_c[(int64_t)i * E + e];
+    }
+  red_p[tid] = p;
+  red_c[tid] = c;
+  __syncthreads();
+  double term = 0.0;
+  if (slice == 0 && e < E) {
+    for (int i = 1; i < slices; ++i) {
+      p += red_p[i * width + e];
+      c += red_c[i * width + e];
+    }
+    counts[e] = c;
+    term = (double)c * p;
+  }
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) term += __shfl_xor(term, m);
+  if (tid % kWave == 0) sums[tid / kWave] = term;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < kJoin / kWave; ++i) term += sums[i];
+    *kept = n;
+    *loss = n ? (float)(term * E / ((double)n * (double)n * top_k)) : 0.f;
+  }
+}
+
+template <typename T, int G, int C>
+__global__ __launch_bounds__(kBlock) void balance_bwd_kernel(const T *__restrict__ logits, int64_t ld,
+                                                             const uint8_t *__restrict__ mask, int64_t rows, int E,
+                                                             int top_k, const int64_t *__restrict__ counts,
+                                                             const int64_t *__restrict__ kept,
+                                                             const float *__restrict__ grad, T *__restrict__ out) {
+  constexpr int V = Row<T, G, C>::V, kRows = kBlock / G;
+  const int t = lane_id() % G;
+  const double n = (double)*kept;
+  const float share = n > 0 ? (float)(1.0 / (n * top_k)) : 0.f;
+  const float scale = n > 0 ? (float)((double)*grad * E / n) : 0.f;
+  float f[C][V];
+#pragma unroll
+  for (int j = 0; j < C; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = (t + G * j) * V + i;
+      f[j][i] = e < E ? (float)counts[e] * share : 0.f;
+    }
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t r = r0 + threadIdx.x / G;
+    const bool use = r < rows && (!mask || mask[r]);
+    Row<T, G, C> row;
+    row.load(logits + (use ? r : 0) * ld, use ? E : 0, t);
+    const float m = row.max();
+    const bool keep = use && m > -INFINITY;
+    float p[C][V];
+    row.softmax(keep ? m : 0.f, p);
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) dot += f[j][i] * p[j][i];
+    dot = group_sum<G>(dot);
+    if (r >= rows) continue;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int e0 = (t + G * j) * V;
+      T d[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = (T)(keep ? scale * p[j][i] * (f[j][i] - dot) : 0.f);
+      if (e0 + V <= E) {
+        __builtin_memcpy(out + r * E + e0, d, 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (e0 + i < E) out[r * E + e0 + i] = d[i];
+      }
+    }
+  }
+}
+
+struct Call {
+  const void *logits;
+  int64_t ld;
+  const uint8_t *mask;
+  int64_t rows;
+  int E, top_k;
+  float *loss;
+  int64_t *counts, *kept;
+  void *ws;
+  const float *grad;
+  void *out;
+};
+
+size_t a256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Lanes per row and chunks per lane.
+void row_shape(int E, int V, int *G, int *C) {
+  const int chunks = (E + V - 1) / V;
+  *G = 1;
+  while (*G < kWave && *G < chunks) *G *= 2;
+  *C = 1;
+  while (*G * *C < chunks) *C *= 2;
+}
+
+template <typename T, int G, int C>
+void launch(const Call &c, int parts, hipStream_t s) {
+  const T *logits = static_cast<const T *>(c.logits);
+  if (c.out) {
+    const int64_t blocks = ceil_div(c.rows, kBlock / G);
+    hipLaunchKernelGGL((balance_bwd_kernel<T, G, C>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kBlock), 0,
+                       s, logits, c.ld, c.mask, c.rows, c.E, c.top_k, c.counts, c.kept, c.grad,
+                       static_cast<T *>(c.out));
+    return;
+  }
+  float *part_p = static_cast<float *>(c.ws);
+  int32_t *part_c = reinterpret_cast<int32_t *>(part_p + (int64_t)parts * c.E);
+  int32_t *part_n = part_c + (int64_t)parts * c.E;
+  hipLaunchKernelGGL((balance_fwd_kernel<T, G, C>), dim3(parts), dim3(kBlock), 0, s, logits, c.ld, c.mask, c.rows, c.E,
+                     c.top_k, part_p, part_c, part_n);
+  hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(kJoin), 0, s, part_p, part_c, part_n, parts, c.E, c.top_k,
+                     c.loss, c.counts, c.kept);
+}
+
+int parts_of(int64_t rows, int E, int es) {
+  int G, C;
+  row_shape(E, 16 / es, &G, &C);
+  const int64_t blocks = ceil_div(rows, kBlock / G);
+  return (int)(blocks < 1 ? 1 : blocks < kMaxParts ? blocks : kMaxParts);
+}
+
+template <typename T>
+void launch_type(const Call &c, hipStream_t s) {
+  const int parts = parts_of(c.rows, c.E, sizeof(T));
+  int G, C;
+  row_shape(c.E, 16 / (int)sizeof(T), &G, &C);
+#define SFT_BALANCE(g, k) \
+  if (G == g && C == k) return launch<T, g, k>(c, parts, s)
+  SFT_BALANCE(1, 1);
+  SFT_BALANCE(2, 1);
+  SFT_BALANCE(4, 1);
+  SFT_BALANCE(8, 1);
+  SFT_BALANCE(16, 1);
+  SFT_BALANCE(32, 1);
+  SFT_BALANCE(64, 1);
+  SFT_BALANCE(64, 2);
+  if constexpr (sizeof(T) == 4) SFT_BALANCE(64, 4);
+#undef SFT_BALANCE
+}
+
+int run(int dtype, const Call &c, hipStream_t s, const char *who) {
+  ProfScope prof(kProfDenseBalance, s);
+  if (dtype == SFT_TYPE_F32) launch_type<float>(c, s);
+  else if (dtype == SFT_TYPE_F16) launch_type<f16_t>(c, s);
+  else launch_type<bf16_t>(c, s);
+  return check_launch(who);
+}
+
+}  // namespace
+
+size_t balance_fwd_workspace(int dtype, int64_t rows, int E) {
+  const size_t parts = parts_of(rows, E, dtype == SFT_TYPE_F32 ? 4 : 2);
+  return a256(parts * (size_t)E * 8 + parts * 4);
+}
+
+int balance_fwd(int dtype, const void *logits, int64_t ld, const uint8_t *mask, int64_t rows, int E, int top_k,
+                float *loss, int64_t *counts, int64_t *kept, void *ws, hipStream_t s) {
+  return run(dtype, Call{logits, ld, mask, rows, E, top_k, loss, counts, kept, ws, nullptr, nullptr}, s,
+             "sft_balance_fwd");
+}
+
+int balance_bwd(int dtype, const void *logits, int64_t ld, const uint8_t *mask, int64_t rows, int E, int top_k,
+                const int64_t *counts, const int64_t *kept, const float *grad, void *out, hipStream_t s) {
+  return run(dtype,
+             Call{logits, ld, mask, rows, E, top_k, nullptr, const_cast<int64_t *>(counts),
+                  const_cast<int64_t *>(kept), nullptr, grad, out},
+             s, "sft_balance_bwd");
+}
+
+}  // namespace sft

@@ -44,6 +44,8 @@ SFT_ACT_CRELU = 2
 SFT_ACT_SCRELU = 3
 SFT_ACT_SILU = 4
 SFT_ACT_GELU = 5
+SFT_BALANCE_MAX_EXPERTS = 1024
+SFT_DISTILL_MAX_K = 256
 SFT_FEATURES_THREATS = 1
 SFT_FEATURES_HALFKA = 2
 
@@ -133,6 +135,13 @@ SIGNATURES = {
         ctypes.c_int,
         [_i32, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, ctypes.c_size_t,
          _vp]),
+    "sft_balance_fwd_workspace_size": (ctypes.c_int, [_i32, _i64, _i32, ctypes.POINTER(ctypes.c_size_t)]),
+    "sft_balance_fwd": (
+        ctypes.c_int, [_i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "sft_balance_bwd": (ctypes.c_int, [_i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "sft_distill": (
+        ctypes.c_int,
+        [_i32, _vp, _i64, _i32, _vp, _vp, _i32, _i64, _i64, _i32, ctypes.c_float, _vp, _vp, _vp, _vp]),
     "sft_probe_l2_gather": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
     "sft_prof_enable": (ctypes.c_int, [ctypes.c_int]),
     "sft_prof_num_kinds": (ctypes.c_int, []),
@@ -816,6 +825,41 @@ def linear_bwd(dy, deriv, x, w, dx, dw, db, act: int) -> None:
                                     _ptr(dx), _ptr(dw), _ptr(db), M, K, N, act, ws, n.value, _stream(dev)),
                "sft_linear_bwd")
     del keep
+
+
+def balance_fwd(logits, mask, top_k: int, loss, counts, kept) -> None:
+    """loss (float32), counts (int64 [E]) and kept (int64) of the router's 2-D logits; mask bool [T] or None."""
+    T, E = logits.shape
+    code = type_code(logits.dtype)
+    dev = logits.device
+    n = ctypes.c_size_t(0)
+    _check(lib().sft_balance_fwd_workspace_size(code, T, E, ctypes.byref(n)), "sft_balance_fwd_workspace_size")
+    with torch.cuda.device(dev):
+        keep, ws = _scratch(n.value, dev)
+        _check(lib().sft_balance_fwd(code, _ptr(logits), _rows(logits), _ptr(mask), T, E, top_k, _ptr(loss),
+                                     _ptr(counts), _ptr(kept), ws, n.value, _stream(dev)), "sft_balance_fwd")
+    del keep
+
+
+def balance_bwd(logits, mask, top_k: int, counts, kept, grad_loss, grad_logits) -> None:
+    """grad_logits (dense) of balance_fwd's loss times grad_loss (float32 on the device)."""
+    T, E = logits.shape
+    dev = logits.device
+    with torch.cuda.device(dev):
+        _check(lib().sft_balance_bwd(type_code(logits.dtype), _ptr(logits), _rows(logits), _ptr(mask), T, E, top_k,
+                                     _ptr(counts), _ptr(kept), _ptr(grad_loss), _ptr(grad_logits), _stream(dev)),
+               "sft_balance_bwd")
+
+
+def distill(student, teacher, indices, temperature: float, row_weight, loss, grad_student) -> None:
+    """loss (float32 [R]) and grad_student (dense), each may be None, of 2-D logits and a teacher's dense top ones."""
+    R, V = student.shape
+    dev = student.device
+    with torch.cuda.device(dev):
+        _check(lib().sft_distill(type_code(student.dtype), _ptr(student), _rows(student), type_code(teacher.dtype),
+                                 _ptr(teacher), _ptr(indices), indices.element_size(), R, V, teacher.shape[1],
+                                 temperature, _ptr(row_weight), _ptr(loss), _ptr(grad_student), _stream(dev)),
+               "sft_distill")
 
 
 # ---- per-launch kernel timing ----

@@ -21,6 +21,7 @@ from torch import Tensor, autograd
 from sft_amd import _native
 
 from . import ops  # noqa: F401  (registers torch.ops.sft.*)
+from .rows import dense_rows
 
 ACTIVATIONS = {
     "none": _native.SFT_ACT_NONE,
@@ -32,22 +33,12 @@ ACTIVATIONS = {
 }
 
 
-def _dense_rows(t: Tensor | None) -> Tensor | None:
-    """t, or a copy where its rows are not dense, overlap or lie in descending order."""
-    if t is None or t.is_contiguous():
-        return t
-    rows, cols = t.shape
-    if (cols == 1 or t.stride(1) == 1) and (rows == 1 or t.stride(0) >= cols):
-        return t
-    return t.contiguous()
-
-
 class FusedLinearFunction(autograd.Function):
     """apply(x [M, K], weight [N, K], bias [N] or None, residual [M, N] or None, act code) -> y [M, N]."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        x, weight, residual = _dense_rows(x), _dense_rows(weight), _dense_rows(residual)
+        x, weight, residual = dense_rows(x), dense_rows(weight), dense_rows(residual)
         bias = None if bias is None else bias.contiguous()
         y, deriv = torch.ops.sft.linear_fwd(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, deriv)
@@ -61,7 +52,7 @@ class FusedLinearFunction(autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            dx, dw, db = torch.ops.sft.linear_bwd(_dense_rows(grad_y), deriv, x, weight, ctx.act, *need[:3])
+            dx, dw, db = torch.ops.sft.linear_bwd(dense_rows(grad_y), deriv, x, weight, ctx.act, *need[:3])
         return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None,
                 grad_y if need[3] else None, None)
 
@@ -92,7 +83,7 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
         y = FusedLinearFunction.apply(x, weight, bias, residual, act)
     else:
         # nothing to record: straight to the library
-        x, weight, residual = _dense_rows(x), _dense_rows(weight), _dense_rows(residual)
+        x, weight, residual = dense_rows(x), dense_rows(weight), dense_rows(residual)
         y = torch.empty(x.shape[0], N, dtype=x.dtype, device=x.device)
         _native.linear_fwd(x, weight, None if bias is None else bias.contiguous(), residual, y, None, act)
     return y if len(lead) == 1 else y.view(*lead, N)

@@ -79,3 +79,63 @@ def worst(got, ref):
     off = (got - value).abs()
     assert torch.isfinite(off).all()
     return (off / bound.clamp(min=1e-300)).max().item()
+
+
+def balance(logits, mask, top_k, grad=1.0):
+    """(loss, counts, dlogits), the floats with bounds; logits [T, E] on the CPU in their own type."""
+    dtype, (T, E) = logits.dtype, logits.shape
+    x = logits.double()
+    keep = torch.ones(T, dtype=torch.bool) if mask is None else mask.clone()
+    keep &= (x > -math.inf).any(1)
+    rows = x[keep]
+    n = len(rows)
+    counts = torch.zeros(E, dtype=torch.int64)
+    for row in rows:  # the top_k largest, equal ones from the front, none at -inf
+        order = sorted(range(E), key=lambda e: (-row[e].item(), e))[:top_k]
+        for e in order:
+            counts[e] += row[e].item() > -math.inf
+    p = torch.softmax(rows, 1)
+    spread = torch.where(rows > -math.inf, rows.max(1, keepdim=True).values - rows, torch.zeros_like(rows)).amax(
+        1, keepdim=True) if n else torch.zeros(0, 1, dtype=torch.float64)
+    relp = (2 * spread + E + 16) * U32
+    f = counts.double() / (max(n, 1) * top_k)
+    mean = p.sum(0) / max(n, 1)
+    merr = (relp * p).sum(0) / max(n, 1) + (T / 2048 + 16) * U32 * mean
+    loss = E * (f * mean).sum()
+    lerr = E * (f * merr).sum() + 8 * U32 * loss
+    d = torch.zeros(T, E, dtype=torch.float64)
+    derr = torch.zeros(T, E, dtype=torch.float64)
+    scale = abs(grad) * E / max(n, 1)
+    dot = (f * p).sum(1, keepdim=True)
+    d[keep] = grad * E / max(n, 1) * p * (f - dot)
+    derr[keep] = scale * p * (2 * relp * (f - dot).abs() + (relp + (E + 8) * U32) * dot + 8 * U32 * f)
+    return (loss, lerr + TINY[torch.float32]), counts, (d, torch.where(keep[:, None], rounded(derr, d, dtype), 0.0))
+
+
+def distill(s, t, i, tau, weight=None):
+    """loss [R] and ds [R, V] with bounds; inputs on the CPU."""
+    dtype, (R, V), k = s.dtype, s.shape, t.shape[1]
+    x, loss, lerr = s.double() / tau, torch.zeros(R, dtype=torch.float64), torch.zeros(R, dtype=torch.float64)
+    ds, derr = torch.zeros(R, V, dtype=torch.float64), torch.zeros(R, V, dtype=torch.float64)
+    w = torch.ones(R, dtype=torch.float64) if weight is None else weight.double()
+    for r in range(R):
+        full = (i[r] >= 0) & (i[r] < V) & (t[r].double() > -math.inf)
+        if not full.any() or not (x[r] > -math.inf).any():
+            continue
+        tt, at = t[r][full].double() / tau, i[r][full].long()
+        q, p = torch.softmax(tt, 0), torch.softmax(x[r], 0)
+        logq, logp = torch.log_softmax(tt, 0), torch.log_softmax(x[r], 0)
+        alive = x[r][x[r] > -math.inf]
+        span = (alive.max() - alive.min()).item()
+        relp = (4 * span + V / 64 + 24) * U32
+        relq = (2 * (tt.max() - tt.min()).item() + k + 16) * U32
+        used = q > 0
+        terms = q[used] * (logq[used] - logp[at][used])
+        loss[r] = tau * tau * terms.sum()
+        size = (q[used] * (tt[used].abs() + tt.abs().max() + logq[used].abs() + x[r][at][used].abs())).sum()
+        lerr[r] = tau * tau * (relq * size + (k + 16) * U32 * size + relp + 8 * U32 * (alive.abs().max() + math.log(V) + 1))
+        each = torch.zeros(V, dtype=torch.float64).index_add_(0, at, q)
+        ds[r] = w[r] * tau * (p - each)
+        derr[r] = w[r].abs() * tau * (relp * p + relq * each + (k + 8) * U32 * (p + each))
+    some = (derr != 0).any(1, keepdim=True)
+    return (loss, lerr), (ds, torch.where(some, rounded(derr, ds, dtype), torch.zeros_like(derr)))
