@@ -473,7 +473,10 @@ int sft_quantize_i16(const float *x, int64_t n, float scale, int16_t *out, void 
  * The backward reads dy ([M, N], rows lddy apart) and the forward's deriv and writes
  * dense dx [M, K], dw [N, K] and db [N], each NULL if not wanted (the residual's
  * gradient is dy).  Results do not vary from run to run.
- * K and N in [1, 2^26], M in [0, 2^30]; M = 0 is no rows: an empty y, zero dw and db.
+ * The products read matrices in place whose rows are 16-byte aligned and a multiple
+ * of 16 bytes long, and aligned copies of the others; the workspace sizes are for
+ * dense, 16-byte aligned tensors, with SFT_LINEAR_COPY for any.
+ * K and N in [1, 2^21], M in [0, 2^30]; M = 0 is no rows: an empty y, zero dw and db.
  */
 #define SFT_TYPE_F32 0
 #define SFT_TYPE_F16 1
@@ -484,13 +487,15 @@ int sft_quantize_i16(const float *x, int64_t n, float scale, int16_t *out, void 
 #define SFT_ACT_SCRELU 3 /* clamp(z, 0, 1)^2           */
 #define SFT_ACT_SILU 4   /* z / (1 + exp(-z))          */
 #define SFT_ACT_GELU 5   /* z Phi(z), the exact form   */
-int sft_linear_fwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, size_t *bytes);
+#define SFT_LINEAR_COPY 0x1u
+int sft_linear_fwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, uint32_t flags,
+                                  size_t *bytes);
 int sft_linear_fwd(int32_t dtype, const void *x, int64_t ldx, const void *w, int64_t ldw,
                    const void *bias, const void *residual, int64_t ldr, void *y, int64_t ldy,
                    void *deriv, int64_t M, int64_t K, int64_t N, int32_t act, void *workspace,
                    size_t workspace_bytes, void *stream);
 int sft_linear_bwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, int32_t act,
-                                  size_t *bytes);
+                                  uint32_t flags, size_t *bytes);
 int sft_linear_bwd(int32_t dtype, const void *dy, int64_t lddy, const void *deriv, const void *x,
                    int64_t ldx, const void *w, int64_t ldw, void *dx, void *dw, void *db, int64_t M,
                    int64_t K, int64_t N, int32_t act, void *workspace, size_t workspace_bytes,

@@ -63,11 +63,14 @@ int probe_l2_gather(const float *table, int64_t table_rows, int rounds, int bloc
 int encode_features(const uint8_t *boards, const uint8_t *stm, int64_t B, const int32_t *comps, int ncomp,
                     int32_t *white, int32_t *black, int K, float *us, int64_t *psqt, int64_t *ls, int32_t *count_w,
                     int32_t *count_b, hipStream_t s);
-size_t linear_fwd_workspace(int dtype, int64_t M, int64_t K, int64_t N);
+size_t linear_fwd_workspace(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t M, int64_t K,
+                            int64_t N, bool copied);
 int linear_fwd(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
                const void *residual, int64_t ldr, void *y, int64_t ldy, void *deriv, int64_t M, int64_t K, int64_t N,
                int act, void *ws, hipStream_t s);
-size_t linear_bwd_workspace(int dtype, int64_t M, int64_t K, int64_t N, int act);
+size_t linear_bwd_workspace(int dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w,
+                            int64_t ldw, bool dx, bool dw, bool db, int64_t M, int64_t K, int64_t N, int act,
+                            bool copied);
 int linear_bwd(int dtype, const void *dy, int64_t lddy, const void *deriv, const void *x, int64_t ldx, const void *w,
                int64_t ldw, void *dx, void *dw, void *db, int64_t M, int64_t K, int64_t N, int act, void *ws,
                hipStream_t s);
@@ -264,7 +267,7 @@ const char *const kKindNames[] = {
     "bwd_bias_final",   "bwd_atomic_scatter", "bwd_zero_fill",      "fwd_i16_gather",     "quantize_i16",
     "fwd_tile_relayout", "fwd_f32_tiled_gather", "bwd_tiled_gather", "fwd_i16_tiled_gather",
     "fwd_fold_relayout", "bwd_virtual_reduce", "bwd_epilogue", "ranger22_update", "encode_features", "leb128_encode",
-    "probe_l2_gather", "fwd_rank_lists", "dense_product", "dense_act_bwd",
+    "probe_l2_gather", "fwd_rank_lists", "dense_product", "dense_act_bwd", "dense_aligned_copy",
     "dense_balance", "dense_distill",
 };
 static_assert(sizeof(kKindNames) / sizeof(kKindNames[0]) == kProfNumKinds, "one name per profiling kind");
@@ -306,11 +309,11 @@ bool bad_sizes(int64_t B, int32_t K, int64_t N, int32_t L, std::string &why) {
 
 // A linear layer's sizes, type and activation.
 bool bad_linear(int32_t dtype, int64_t M, int64_t K, int64_t N, int32_t act, std::string &why) {
-  constexpr int64_t kMostRows = (int64_t)1 << 30, kMost = (int64_t)1 << 26;
+  constexpr int64_t kMostRows = (int64_t)1 << 30, kMost = (int64_t)1 << 21;
   if (dtype < SFT_TYPE_F32 || dtype > SFT_TYPE_BF16) why = "unknown type";
   else if (act < SFT_ACT_NONE || act > SFT_ACT_GELU) why = "unknown activation";
   else if (M < 0 || M > kMostRows) why = "M must be in [0, 2^30]";
-  else if (K < 1 || K > kMost || N < 1 || N > kMost) why = "K and N must be in [1, 2^26]";
+  else if (K < 1 || K > kMost || N < 1 || N > kMost) why = "K and N must be in [1, 2^21]";
   else if (M * K >= (1ll << 40) || M * N >= (1ll << 40) || K * N >= (1ll << 40)) why = "tensor too large";
   else return false;
   return true;
@@ -812,13 +815,14 @@ int sft_encode_features(const uint8_t *boards, const uint8_t *side_to_move, int6
                          psqt_indices, layer_stack_indices, white_count, black_count, (hipStream_t)stream);
 }
 
-int sft_linear_fwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, size_t *bytes) {
+int sft_linear_fwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, uint32_t flags, size_t *bytes) {
   clear_error();
   const char *who = "sft_linear_fwd_workspace_size";
   std::string why;
   if (!bytes) return fail(SFT_EINVAL, std::string(who) + ": null pointer");
+  if (flags & ~SFT_LINEAR_COPY) return fail(SFT_EINVAL, std::string(who) + ": unknown flags");
   if (bad_linear(dtype, M, K, N, SFT_ACT_NONE, why)) return fail(SFT_EINVAL, std::string(who) + ": " + why);
-  *bytes = linear_fwd_workspace(dtype, M, K, N);
+  *bytes = linear_fwd_workspace(dtype, nullptr, K, nullptr, K, M, K, N, flags & SFT_LINEAR_COPY);
   return SFT_OK;
 }
 
@@ -835,20 +839,23 @@ int sft_linear_fwd(int32_t dtype, const void *x, int64_t ldx, const void *w, int
     return fail(SFT_EINVAL, std::string(who) + ": a row stride is smaller than its row, or 2^40 or more");
   if (misaligned(dtype, {x, w, bias, residual, y, deriv}))
     return fail(SFT_EINVAL, std::string(who) + ": a tensor is not aligned to its type");
-  const size_t need = linear_fwd_workspace(dtype, M, K, N);
+  const size_t need = linear_fwd_workspace(dtype, x, ldx, w, ldw, M, K, N, false);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256))
     return fail(SFT_EWORKSPACE, std::string(who) + ": needs " + std::to_string(need) + " bytes, 256-byte aligned");
   return linear_fwd(dtype, x, ldx, w, ldw, bias, residual, ldr, y, ldy, deriv, M, K, N, act, workspace,
                     (hipStream_t)stream);
 }
 
-int sft_linear_bwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, int32_t act, size_t *bytes) {
+int sft_linear_bwd_workspace_size(int32_t dtype, int64_t M, int64_t K, int64_t N, int32_t act, uint32_t flags,
+                                  size_t *bytes) {
   clear_error();
   const char *who = "sft_linear_bwd_workspace_size";
   std::string why;
   if (!bytes) return fail(SFT_EINVAL, std::string(who) + ": null pointer");
+  if (flags & ~SFT_LINEAR_COPY) return fail(SFT_EINVAL, std::string(who) + ": unknown flags");
   if (bad_linear(dtype, M, K, N, act, why)) return fail(SFT_EINVAL, std::string(who) + ": " + why);
-  *bytes = linear_bwd_workspace(dtype, M, K, N, act);
+  *bytes = linear_bwd_workspace(dtype, nullptr, N, nullptr, K, nullptr, K, true, true, true, M, K, N, act,
+                                flags & SFT_LINEAR_COPY);
   return SFT_OK;
 }
 
@@ -865,7 +872,8 @@ int sft_linear_bwd(int32_t dtype, const void *dy, int64_t lddy, const void *deri
     return fail(SFT_EINVAL, std::string(who) + ": a row stride is smaller than its row, or 2^40 or more");
   if (misaligned(dtype, {dy, deriv, x, w, dx, dw, db}))
     return fail(SFT_EINVAL, std::string(who) + ": a tensor is not aligned to its type");
-  const size_t need = M > 0 ? linear_bwd_workspace(dtype, M, K, N, act) : 0;
+  const size_t need =
+      linear_bwd_workspace(dtype, dy, lddy, x, ldx, w, ldw, dx != nullptr, dw != nullptr, db != nullptr, M, K, N, act, false);
   if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256))
     return fail(SFT_EWORKSPACE, std::string(who) + ": needs " + std::to_string(need) + " bytes, 256-byte aligned");
   return linear_bwd(dtype, dy, lddy, deriv, x, ldx, w, ldw, dx, dw, db, M, K, N, act, workspace, (hipStream_t)stream);

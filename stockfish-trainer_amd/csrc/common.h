@@ -86,6 +86,7 @@ enum ProfKind : int {
   kProfFwdRanks,
   kProfDenseProduct,
   kProfDenseActBwd,
+  kProfDenseAlign,
   kProfDenseBalance,
   kProfDenseDistill,
   kProfNumKinds

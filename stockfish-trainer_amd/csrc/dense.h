@@ -8,6 +8,8 @@ namespace sft {
 namespace dense {
 
 enum Layout { kForward = 0, kInputGrad = 1, kWeightGrad = 2 };
+// Tiles of a product: 64 x 128, 128 x 128 and, of 16-bit types, 256 x 256.
+enum TileKind { kTile64 = 0, kTile128 = 1, kTile256 = 2 };
 
 // What becomes of a product's sums: y = residual + act(sum + bias), rounded once.
 struct Epilogue {
@@ -17,28 +19,34 @@ struct Epilogue {
   void *deriv;           // dense [M, N] of act', or null
   int64_t ldr, ldy;
   int act;
-  bool vec;  // rows of bias, residual, y and deriv take 4-element accesses
+  bool vec;  // bias, residual, y and deriv take 16-byte accesses (of few rows: of 4 elements)
 };
 
-// C[M, N] = sum over K of A(m, k) B(n, k).
+// C[M, N] = sum over K of A(m, k) B(n, k).  Operands padded to whole chunks have ma >= M
+// rows or nb >= N columns, and ka, kb <= K of the k's each; what lacks is zero.
 struct Gemm {
   const void *a, *b;
   int64_t lda, ldb;
   int M, N, K;
-  int tiles_m, tiles_n;
+  int ma, nb, ka, kb;
+  int tile, tiles_m, tiles_n;
   int splits, split_k;  // k per split, whole stages
   float *part;          // [splits][M][N] when splits > 1
-  bool direct;          // both operands take aligned 16-byte copies
   Epilogue epi;
 };
 
 struct ActBwd {
   const void *dy, *deriv;  // deriv null: dz is dy, only the sums are made
-  void *dz;
-  float *part;  // [parts][N] or null
-  int64_t lddy, M, rows;
+  void *dz;                // rows lddz apart, whole chunks
+  float *part;             // [parts][N] or null
+  int64_t lddy, lddz, M, rows;
   int N, parts, tx;
-  bool vec;
+};
+
+struct Copy {
+  const void *from;
+  void *to;
+  int64_t ld, to_ld, rows, cols;  // elements
 };
 
 template <typename T>
@@ -47,6 +55,8 @@ template <typename T>
 int launch_rows(const Gemm &g, hipStream_t s);
 template <typename T>
 int launch_act_bwd(const ActBwd &p, void *db, hipStream_t s);
+template <typename T>
+int launch_align(const Copy &a, const Copy &b, hipStream_t s);
 
 }  // namespace dense
 }  // namespace sft

@@ -10,52 +10,149 @@ typedef _Float16 f16_t;
 
 namespace {
 
-constexpr int kStage = 128;          // bytes of k per pipeline stage
-constexpr int kTile = 128;           // rows and columns of a tile
-constexpr int64_t kRowsMost = 64;    // rows the row kernel takes
-constexpr int64_t kSlots = 2 * 256;  // tile workgroups the card holds at once
+constexpr int kStage = 64;         // bytes of k per pipeline stage
+constexpr int64_t kRowsMost = 64;  // rows the row kernel takes
+constexpr int64_t kCus = 256;
+constexpr int64_t kStrideMost = (int64_t)1 << 23;  // bytes: a tile's rows stay within 31-bit offsets
 
 size_t a256(size_t n) { return (n + 255) & ~(size_t)255; }
 int64_t type_size(int dtype) { return dtype == SFT_TYPE_F32 ? 4 : 2; }
+int64_t padded(int64_t n, int64_t es) { return (n + 16 / es - 1) & ~(16 / es - 1); }
 
-// A product with few tiles and a long k is split along k, so that the card is full,
-// as long as every part has at least 8 stages.
-int splits_of(int dtype, int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = ceil_div(M, kTile) * ceil_div(N, kTile);
-  const int64_t stages = ceil_div(K * type_size(dtype), kStage);
-  int64_t s = kSlots / tiles;
-  if (s > stages / 8) s = stages / 8;
-  if (s < 1) return 1;
-  const int64_t per = ceil_div(stages, s);
-  return (int)ceil_div(stages, per);
+#define SFT_DENSE_CALL(dtype, F, ...)                         \
+  (dtype == SFT_TYPE_F32   ? F<float>(__VA_ARGS__)            \
+   : dtype == SFT_TYPE_F16 ? F<f16_t>(__VA_ARGS__)            \
+                           : F<bf16_t>(__VA_ARGS__))
+
+// How a product is cut into tiles, and its k into parts whose sums one more launch
+// adds.  Taken is what a model of the time says is least: a CU works through its share
+// of the tiles at a time per stage that was measured with many of them (below, us, at
+// 8192^3 and 65536 x 1040 x 4096), each round of workgroups adds its first copies'
+// latency and its results' stores, and partials are written and read at 4 TB/s.
+struct Cut {
+  int tile, tiles_m, tiles_n, splits, split_k;
+};
+struct TileCost {
+  int rows, cols, slots;              // slots: workgroups the card holds at once
+  double stage[2], alone[2], round;   // us a stage of 16-bit types and of binary32, with many and one per CU
+};
+constexpr TileCost kTiles[3] = {{64, 128, 768, {0.17, 0.50}, {0.26, 0.57}, 4.0},
+                                {128, 128, 768, {0.29, 0.95}, {0.42, 1.00}, 5.0},
+                                {256, 256, 256, {0.84, 0.0}, {0.84, 0.0}, 8.0}};
+Cut cut_of(int dtype, int64_t M, int64_t N, int64_t K) {
+  const int64_t es = type_size(dtype), stages = ceil_div(K * es, kStage);
+  Cut best = {};
+  double least = 0.0;
+  for (int t = 0; t < (es == 2 ? 3 : 2); ++t) {
+    const TileCost &c = kTiles[t];
+    const int64_t tm = ceil_div(M, c.rows), tn = ceil_div(N, c.cols), n = tm * tn;
+    for (int64_t s = 1; s <= 64 && s * 8 <= stages + 7; ++s) {
+      const int64_t per = ceil_div(stages, s), parts = ceil_div(stages, per);
+      if (parts != s) continue;
+      const int64_t load = ceil_div(n * s, kCus);
+      const double stage = load == 1 ? c.alone[es == 4] : (double)load * c.stage[es == 4];
+      double cost = (double)per * stage + (double)ceil_div(n * s, c.slots) * c.round;
+      if (s > 1) cost += 4.0 + (double)s * (double)M * (double)N * 8.0 / 4e6;
+      if (best.splits && cost >= least) continue;
+      least = cost;
+      best = Cut{t, (int)tm, (int)tn, (int)s, (int)(per * (kStage / es))};
+    }
+  }
+  return best;
 }
 
 size_t part_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-  const int s = splits_of(dtype, M, N, K);
+  const int s = cut_of(dtype, M, N, K).splits;
   return s > 1 ? a256((size_t)s * M * N * 4) : 0;
 }
 
-bool rows16(const void *p, int64_t ld, int64_t es) { return ((uintptr_t)p | (uintptr_t)(ld * es)) % 16 == 0; }
-bool rows4(const void *p, int64_t ld, int64_t es) { return !p || ((uintptr_t)p | (uintptr_t)(ld * es)) % (4 * es) == 0; }
+// A matrix that a product reads: rows of dense elements.
+struct Matrix {
+  const void *p;
+  int64_t ld, rows, cols;
+  // Whole aligned chunks with a stride that tiles can address: read in place.
+  bool direct(int64_t es) const {
+    return ((uintptr_t)p | (uintptr_t)(ld * es)) % 16 == 0 && cols % (16 / es) == 0 && ld * es <= kStrideMost;
+  }
+  size_t copy_bytes(int64_t es) const { return a256((size_t)rows * padded(cols, es) * es); }
+};
 
-int run_gemm(int dtype, Gemm &g, int layout, hipStream_t s) {
-  const int64_t es = type_size(dtype), epc = 16 / es;
+// Takes pieces of the workspace.
+struct Scratch {
+  char *at;
+  void *take(size_t n) {
+    char *p = at;
+    at += n;
+    return p;
+  }
+};
+
+// Replaces what is not read in place by aligned copies, in one launch.
+int align(int dtype, Matrix *a, Matrix *b, Scratch &ws, hipStream_t s) {
+  const int64_t es = type_size(dtype);
+  Copy c[2] = {};
+  int n = 0;
+  Matrix *m[2] = {a, b};
+  for (Matrix *x : m) {
+    if (!x || x->direct(es)) continue;
+    const int64_t ld = padded(x->cols, es);
+    void *to = ws.take(x->copy_bytes(es));
+    c[n++] = Copy{x->p, to, x->ld, ld, x->rows, x->cols};
+    *x = Matrix{to, ld, x->rows, ld};
+  }
+  if (!n) return SFT_OK;
+  ProfScope prof(kProfDenseAlign, s);
+  return SFT_DENSE_CALL(dtype, launch_align, c[0], c[1], s);
+}
+
+// Whether the epilogue may access V elements at once.
+bool epilogue_vec(const Epilogue &e, int64_t N, int64_t es, int64_t V) {
+  auto ok = [&](const void *p, int64_t ld) { return !p || ((uintptr_t)p | (uintptr_t)(ld * es)) % (V * es) == 0; };
+  return N % V == 0 && ok(e.y, e.ldy) && ok(e.bias, 0) && ok(e.residual, e.ldr) && ok(e.deriv, 0);
+}
+
+// C [M, N] of operands that are read in place.
+int run_gemm(int dtype, int layout, const Matrix &a, const Matrix &b, int64_t M, int64_t N, int64_t K,
+             const Epilogue &epi, Scratch ws, hipStream_t s) {
+  const int64_t es = type_size(dtype);
   const bool ak = layout != kWeightGrad, bk = layout == kForward;
-  // A direct copy moves whole aligned chunks, with 32-bit offsets inside a tile.
-  g.direct = rows16(g.a, g.lda, es) && rows16(g.b, g.ldb, es) && (ak ? g.K : g.M) % epc == 0 &&
-             (bk ? g.K : g.N) % epc == 0 && g.lda * es < (1 << 22) && g.ldb * es < (1 << 22);
-  g.epi.vec = g.N % 4 == 0 && rows4(g.epi.y, g.epi.ldy, es) && rows4(g.epi.bias, 0, es) &&
-              rows4(g.epi.residual, g.epi.ldr, es) && rows4(g.epi.deriv, 0, es);
-  g.tiles_m = (int)ceil_div(g.M, kTile);
-  g.tiles_n = (int)ceil_div(g.N, kTile);
-  g.splits = splits_of(dtype, g.M, g.N, g.K);
-  const int64_t stages = ceil_div(g.K * es, kStage);
-  g.split_k = (int)(ceil_div(stages, g.splits) * (kStage / es));
-  if (g.splits == 1) g.part = nullptr;
+  Gemm g = {};
+  g.a = a.p;
+  g.b = b.p;
+  g.lda = a.ld;
+  g.ldb = b.ld;
+  g.M = (int)M;
+  g.N = (int)N;
+  g.K = (int)K;
+  g.ma = (int)(ak ? a.rows : a.cols);
+  g.ka = (int)(ak ? a.cols : a.rows);
+  g.nb = (int)(bk ? b.rows : b.cols);
+  g.kb = (int)(bk ? b.cols : b.rows);
+  if (g.K < g.ka) g.K = g.ka;
+  if (g.K < g.kb) g.K = g.kb;
+  g.epi = epi;
+  g.epi.vec = epilogue_vec(epi, N, es, 16 / es);
+  const Cut c = cut_of(dtype, M, N, K);
+  g.tile = c.tile;
+  g.tiles_m = c.tiles_m;
+  g.tiles_n = c.tiles_n;
+  g.splits = c.splits;
+  g.split_k = c.split_k;
+  g.part = c.splits > 1 ? static_cast<float *>(ws.take(0)) : nullptr;
   ProfScope prof(kProfDenseProduct, s);
-  if (dtype == SFT_TYPE_F32) return launch_gemm<float>(g, layout, s);
-  if (dtype == SFT_TYPE_F16) return launch_gemm<f16_t>(g, layout, s);
-  return launch_gemm<bf16_t>(g, layout, s);
+  return SFT_DENSE_CALL(dtype, launch_gemm, g, layout, s);
+}
+
+// The shape of the activation's backward and bias sums: about 1024 workgroups.
+void shape_act_bwd(int dtype, int64_t M, int64_t N, ActBwd &p) {
+  const int64_t chunks = ceil_div(N, 16 / type_size(dtype));
+  p.M = M;
+  p.N = (int)N;
+  p.tx = 1;
+  while (p.tx < kWave && p.tx < chunks) p.tx *= 2;
+  const int64_t ty = kBlock / p.tx, want = ceil_div(1024, ceil_div(chunks, p.tx));
+  p.rows = ceil_div(ceil_div(M, want), ty) * ty;
+  p.parts = (int)ceil_div(M, p.rows);
 }
 
 __global__ __launch_bounds__(kBlock) void zero16_kernel(uint16_t *p, int64_t n) {
@@ -67,19 +164,7 @@ void zero16(void *p, int64_t n, hipStream_t s) {
                      static_cast<uint16_t *>(p), n);
 }
 
-// The shape of the activation's backward and bias sums: about 1024 workgroups.
-void shape_act_bwd(int dtype, int64_t M, int64_t N, ActBwd &p) {
-  const int64_t V = 16 / type_size(dtype);
-  p.M = M;
-  p.N = (int)N;
-  p.vec = N % V == 0;
-  const int64_t cols = p.vec ? N / V : N;
-  p.tx = 1;
-  while (p.tx < kWave && p.tx < cols) p.tx *= 2;
-  const int64_t ty = kBlock / p.tx, want = ceil_div(1024, ceil_div(cols, p.tx));
-  p.rows = ceil_div(ceil_div(M, want), ty) * ty;
-  p.parts = (int)ceil_div(M, p.rows);
-}
+size_t copy_bytes(const Matrix &m, int64_t es, bool copied) { return copied || !m.direct(es) ? m.copy_bytes(es) : 0; }
 
 }  // namespace
 
@@ -87,47 +172,57 @@ void shape_act_bwd(int dtype, int64_t M, int64_t N, ActBwd &p) {
 
 using namespace dense;
 
-size_t linear_fwd_workspace(int dtype, int64_t M, int64_t K, int64_t N) {
-  return M <= kRowsMost ? 0 : part_bytes(dtype, M, N, K);
+// Workspace of the forward of these operands; copied: whatever their alignment.
+size_t linear_fwd_workspace(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t M, int64_t K,
+                            int64_t N, bool copied) {
+  if (M <= kRowsMost) return 0;
+  const int64_t es = type_size(dtype);
+  return copy_bytes(Matrix{x, ldx, M, K}, es, copied) + copy_bytes(Matrix{w, ldw, N, K}, es, copied) +
+         part_bytes(dtype, M, N, K);
 }
 
 int linear_fwd(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
                const void *residual, int64_t ldr, void *y, int64_t ldy, void *deriv, int64_t M, int64_t K, int64_t N,
-               int act, void *ws, hipStream_t s) {
-  Gemm g = {};
-  g.a = x;
-  g.b = w;
-  g.lda = ldx;
-  g.ldb = ldw;
-  g.M = (int)M;
-  g.N = (int)N;
-  g.K = (int)K;
-  g.part = static_cast<float *>(ws);
-  g.epi = Epilogue{bias, residual, y, act == SFT_ACT_NONE ? nullptr : deriv, ldr, ldy, act, false};
+               int act, void *workspace, hipStream_t s) {
+  Epilogue epi{bias, residual, y, act == SFT_ACT_NONE ? nullptr : deriv, ldr, ldy, act, false};
   if (M <= kRowsMost) {
-    const int64_t es = type_size(dtype);
-    g.epi.vec = N % 4 == 0 && rows4(y, ldy, es) && rows4(bias, 0, es) && rows4(residual, ldr, es) &&
-                rows4(g.epi.deriv, 0, es);
+    Gemm g = {};
+    g.a = x;
+    g.b = w;
+    g.lda = ldx;
+    g.ldb = ldw;
+    g.M = (int)M;
+    g.N = (int)N;
+    g.K = (int)K;
+    g.epi = epi;
+    g.epi.vec = epilogue_vec(epi, N, type_size(dtype), 4);
     ProfScope prof(kProfDenseProduct, s);
-    if (dtype == SFT_TYPE_F32) return launch_rows<float>(g, s);
-    if (dtype == SFT_TYPE_F16) return launch_rows<f16_t>(g, s);
-    return launch_rows<bf16_t>(g, s);
+    return SFT_DENSE_CALL(dtype, launch_rows, g, s);
   }
-  return run_gemm(dtype, g, kForward, s);
+  Scratch ws{static_cast<char *>(workspace)};
+  Matrix a{x, ldx, M, K}, b{w, ldw, N, K};
+  const int rc = align(dtype, &a, &b, ws, s);
+  return rc ? rc : run_gemm(dtype, kForward, a, b, M, N, K, epi, ws, s);
 }
 
-size_t linear_bwd_workspace(int dtype, int64_t M, int64_t K, int64_t N, int act) {
+size_t linear_bwd_workspace(int dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w,
+                            int64_t ldw, bool dx, bool dw, bool db, int64_t M, int64_t K, int64_t N, int act,
+                            bool copied) {
   if (M == 0) return 0;
+  const int64_t es = type_size(dtype);
   ActBwd p = {};
   shape_act_bwd(dtype, M, N, p);
-  const size_t dz = act == SFT_ACT_NONE ? 0 : a256((size_t)M * N * type_size(dtype));
-  const size_t bias = a256((size_t)p.parts * N * 4);
-  const size_t in = part_bytes(dtype, M, K, N), weight = part_bytes(dtype, N, K, M);
-  return dz + bias + (in > weight ? in : weight);
+  const Matrix g{dy, lddy, M, N};
+  size_t n = act != SFT_ACT_NONE ? g.copy_bytes(es) : dx || dw ? copy_bytes(g, es, copied) : 0;
+  if (db) n += a256((size_t)p.parts * N * 4);
+  if (dx) n += copy_bytes(Matrix{w, ldw, N, K}, es, copied);
+  if (dw) n += copy_bytes(Matrix{x, ldx, M, K}, es, copied);
+  const size_t in = dx ? part_bytes(dtype, M, K, N) : 0, weight = dw ? part_bytes(dtype, N, K, M) : 0;
+  return n + (in > weight ? in : weight);
 }
 
 int linear_bwd(int dtype, const void *dy, int64_t lddy, const void *deriv, const void *x, int64_t ldx, const void *w,
-               int64_t ldw, void *dx, void *dw, void *db, int64_t M, int64_t K, int64_t N, int act, void *ws,
+               int64_t ldw, void *dx, void *dw, void *db, int64_t M, int64_t K, int64_t N, int act, void *workspace,
                hipStream_t s) {
   const int64_t es = type_size(dtype);
   if (M == 0) {  // no rows: the sums are empty
@@ -135,60 +230,33 @@ int linear_bwd(int dtype, const void *dy, int64_t lddy, const void *deriv, const
     if (db) zero16(db, N * es / 2, s);
     return check_launch("sft_linear_bwd");
   }
-  char *at = static_cast<char *>(ws);
+  Scratch ws{static_cast<char *>(workspace)};
+  Matrix dz{dy, lddy, M, N};
   ActBwd p = {};
   shape_act_bwd(dtype, M, N, p);
   p.dy = dy;
   p.lddy = lddy;
-  const void *dz = dy;
-  int64_t lddz = lddy;
   if (act != SFT_ACT_NONE) {
     p.deriv = deriv;
-    p.dz = at;
-    dz = at;
-    lddz = N;
-    at += a256((size_t)M * N * es);
+    p.lddz = padded(N, es);
+    p.dz = ws.take(dz.copy_bytes(es));
+    dz = Matrix{p.dz, p.lddz, M, p.lddz};
   }
-  if (db) p.part = reinterpret_cast<float *>(at);
-  at += a256((size_t)p.parts * N * 4);
+  if (db) p.part = static_cast<float *>(ws.take(a256((size_t)p.parts * N * 4)));
   int rc = SFT_OK;
   if (db || act != SFT_ACT_NONE) {
     ProfScope prof(kProfDenseActBwd, s);
-    rc = dtype == SFT_TYPE_F32   ? launch_act_bwd<float>(p, db, s)
-         : dtype == SFT_TYPE_F16 ? launch_act_bwd<f16_t>(p, db, s)
-                                 : launch_act_bwd<bf16_t>(p, db, s);
-    if (rc) return rc;
+    rc = SFT_DENSE_CALL(dtype, launch_act_bwd, p, db, s);
   }
-  Gemm g = {};
-  g.epi.act = SFT_ACT_NONE;
-  g.part = reinterpret_cast<float *>(at);
-  if (dx) {
-    Gemm in = g;
-    in.a = dz;
-    in.lda = lddz;
-    in.b = w;
-    in.ldb = ldw;
-    in.M = (int)M;
-    in.N = (int)K;
-    in.K = (int)N;
-    in.epi.y = dx;
-    in.epi.ldy = K;
-    rc = run_gemm(dtype, in, kInputGrad, s);
-    if (rc) return rc;
-  }
-  if (dw) {
-    Gemm wt = g;
-    wt.a = dz;
-    wt.lda = lddz;
-    wt.b = x;
-    wt.ldb = ldx;
-    wt.M = (int)N;
-    wt.N = (int)K;
-    wt.K = (int)M;
-    wt.epi.y = dw;
-    wt.epi.ldy = K;
-    rc = run_gemm(dtype, wt, kWeightGrad, s);
-  }
+  Matrix in{x, ldx, M, K}, weight{w, ldw, N, K};
+  if (!rc && (dx || dw)) rc = align(dtype, &dz, dx ? &weight : nullptr, ws, s);
+  if (!rc && dw) rc = align(dtype, &in, nullptr, ws, s);
+  if (!rc && dx)
+    rc = run_gemm(dtype, kInputGrad, dz, weight, M, K, N,
+                  Epilogue{nullptr, nullptr, dx, nullptr, 0, K, SFT_ACT_NONE, false}, ws, s);
+  if (!rc && dw)
+    rc = run_gemm(dtype, kWeightGrad, dz, in, N, K, M,
+                  Epilogue{nullptr, nullptr, dw, nullptr, 0, K, SFT_ACT_NONE, false}, ws, s);
   return rc;
 }
 

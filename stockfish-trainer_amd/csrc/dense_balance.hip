@@ -13,6 +13,7 @@
 // sums over positions stay in registers of the lane that owns the expert; workgroups
 // write partials that one more launch adds in a fixed order, in binary64.
 #include "dense.h"
+#include "dense_reduce.h"
 
 namespace sft {
 
@@ -21,20 +22,12 @@ namespace {
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
-constexpr int kMaxParts = 512;  // workgroups of the forward, two per CU
+using dense::group_max;
+using dense::group_reduce;
+using dense::group_sum;
 
-template <int G>
-__device__ __forceinline__ float group_max(float x) {
-#pragma unroll
-  for (int m = 1; m < G; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
-  return x;
-}
-template <int G>
-__device__ __forceinline__ float group_sum(float x) {
-#pragma unroll
-  for (int m = 1; m < G; m <<= 1) x += __shfl_xor(x, m);
-  return x;
-}
+constexpr int kThreads = 1024;   // of the forward: 16 waves, whose sums leave as one partial
+constexpr int kMaxParts = 256;  // its workgroups, one per CU
 
 // A row's logits: lane t of the group holds the chunks t + G j of V elements.
 // Elements past E are -inf.
@@ -85,16 +78,16 @@ struct Row {
 
 // part_p [parts][E] sums of p, part_c [parts][E] counts, part_n [parts] kept rows.
 template <typename T, int G, int C>
-__global__ __launch_bounds__(kBlock) void balance_fwd_kernel(const T *__restrict__ logits, int64_t ld,
-                                                             const uint8_t *__restrict__ mask, int64_t rows, int E,
-                                                             int top_k, float *__restrict__ part_p,
-                                                             int32_t *__restrict__ part_c,
-                                                             int32_t *__restrict__ part_n) {
-  constexpr int V = Row<T, G, C>::V, kRows = kBlock / G;
-  __shared__ float red_p[kWavesPerBlock][G * C * V];
-  __shared__ int32_t red_c[kWavesPerBlock][G * C * V];
-  __shared__ int32_t red_n[kWavesPerBlock];
-  const int lane = lane_id(), t = lane % G, wave = threadIdx.x / kWave;
+__global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restrict__ logits, int64_t ld,
+                                                               const uint8_t *__restrict__ mask, int64_t rows, int E,
+                                                               int top_k, float *__restrict__ part_p,
+                                                               int32_t *__restrict__ part_c,
+                                                               int32_t *__restrict__ part_n) {
+  constexpr int V = Row<T, G, C>::V, kRows = kThreads / G, kWaves = kThreads / kWave;
+  __shared__ float red_p[kWaves][G * C * V];
+  __shared__ int32_t red_c[kWaves][G * C * V];
+  __shared__ int32_t red_n[kWaves];
+  const int lane = lane_id(), t = lane % G, wave = uniform(threadIdx.x / kWave);
   const uint64_t group = (G == kWave ? ~0ull : ((1ull << (G % kWave)) - 1)) << (lane / G * G);
   float sum[C][V];
   int32_t cnt[C][V], kept = 0;
@@ -105,27 +98,32 @@ __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(const T *__restrict
       sum[j][i] = 0.f;
       cnt[j][i] = 0;
     }
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
-    const int64_t r = r0 + threadIdx.x / G;
-    const bool use = r < rows && (!mask || mask[r]);
-    Row<T, G, C> row;
-    row.load(logits + (use ? r : 0) * ld, use ? E : 0, t);
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
+  Row<T, G, C> row, next;
+  auto use = [&](int64_t i) { return i < rows && (!mask || mask[i]); };
+  bool used = use(r);
+  row.load(logits + (used ? r : 0) * ld, used ? E : 0, t);
+  // the whole wave goes round while any of its rows is left
+  for (int64_t left = rows - (int64_t)blockIdx.x * kRows - wave * (kWave / G); left > 0; left -= step) {
+    const bool use_next = use(r + step);
+    next.load(logits + (use_next ? r + step : 0) * ld, use_next ? E : 0, t);
     const float m = row.max();
-    const bool keep = use && m > -INFINITY;  // the same in all lanes of a group
-    if (keep) {
-      float p[C][V];
-      row.softmax(m, p);
+    const bool keep = used && m > -INFINITY;  // the same in all lanes of a group
+    float p[C][V];
+    row.softmax(keep ? m : 0.f, p);
 #pragma unroll
-      for (int j = 0; j < C; ++j)
+    for (int j = 0; j < C; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[j][i] += p[j][i];
-      kept += t == 0;
-    }
-    // The choice: the largest value left, its lowest element, top_k times.  All lanes
-    // of the wave take part in the shuffles.
+      for (int i = 0; i < V; ++i) sum[j][i] += keep ? p[j][i] : 0.f;
+    kept += keep && t == 0;
+    // The choice: the largest value left, its lowest element, top_k times.
     float best = keep ? m : -INFINITY;
     for (int k = 0; k < top_k; ++k) {
-      if (k > 0) best = keep ? row.max() : -INFINITY;
+      if (k > 0) {
+        best = row.max();
+        if (!keep) best = -INFINITY;
+      }
       bool open = best > -INFINITY;  // still to be found, in order of the elements
 #pragma unroll
       for (int j = 0; j < C; ++j) {
@@ -133,19 +131,22 @@ __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(const T *__restrict
 #pragma unroll
         for (int i = V - 1; i >= 0; --i) first = row.x[j][i] == best ? i : first;
         const uint64_t hits = ballot(open && first < V) & group;
-        if (hits && lane == __builtin_ctzll(hits)) {
+        const bool mine = hits && lane == __builtin_ctzll(hits);
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (i == first) {
-              ++cnt[j][i];
-              row.x[j][i] = -INFINITY;
-            }
+        for (int i = 0; i < V; ++i) {
+          const bool at = mine && i == first;
+          cnt[j][i] += at;
+          row.x[j][i] = at ? -INFINITY : row.x[j][i];
         }
         open = open && !hits;
       }
     }
+    row = next;
+    used = use_next;
+    r += step;
   }
   // Sums over the row groups of the wave, then over the waves.
+  auto add = [](auto a, auto b) { return a + b; };
 #pragma unroll
   for (int j = 0; j < C; ++j)
 #pragma unroll
@@ -160,15 +161,25 @@ __global__ __launch_bounds__(kBlock) void balance_fwd_kernel(const T *__restrict
         red_c[wave][(t + G * j) * V + i] = cnt[j][i];
       }
     }
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) kept += __shfl_xor(kept, m);
+  kept = group_reduce<kWave>(kept, add);
   if (lane == 0) red_n[wave] = kept;
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kBlock) {
-    part_p[(int64_t)blockIdx.x * E + e] = (red_p[0][e] + red_p[1][e]) + (red_p[2][e] + red_p[3][e]);
-    part_c[(int64_t)blockIdx.x * E + e] = (red_c[0][e] + red_c[1][e]) + (red_c[2][e] + red_c[3][e]);
+  for (int e = threadIdx.x; e < E; e += kThreads) {
+    float p = red_p[0][e];
+    int32_t c = red_c[0][e];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      p += red_p[w][e];
+      c += red_c[w][e];
+    }
+    part_p[(int64_t)blockIdx.x * E + e] = p;
+    part_c[(int64_t)blockIdx.x * E + e] = c;
   }
-  if (threadIdx.x == 0) part_n[blockIdx.x] = (red_n[0] + red_n[1]) + (red_n[2] + red_n[3]);
+  if (threadIdx.x == 0) {
+    int32_t n = 0;
+    for (int w = 0; w < kWaves; ++w) n += red_n[w];
+    part_n[blockIdx.x] = n;
+  }
 }
 
 // One workgroup: counts, the number of kept rows and the loss from the partials.
@@ -201,11 +212,13 @@ __global__ __launch_bounds__(kJoin) void balance_join_kernel(const float *__rest
   __syncthreads();
   double p = 0.0;
   int64_t c = 0;
-  if (e < E)
+  if (e < E) {
+#pragma unroll 8
     for (int i = slice; i < parts; i += slices) {
       p += (double)part_p[(int64_t)i * E + e];
       c += part_c[(int64_t)i * E + e];
     }
+  }
   red_p[tid] = p;
   red_c[tid] = c;
   __syncthreads();
@@ -318,8 +331,8 @@ void launch(const Call &c, int parts, hipStream_t s) {
   float *part_p = static_cast<float *>(c.ws);
   int32_t *part_c = reinterpret_cast<int32_t *>(part_p + (int64_t)parts * c.E);
   int32_t *part_n = part_c + (int64_t)parts * c.E;
-  hipLaunchKernelGGL((balance_fwd_kernel<T, G, C>), dim3(parts), dim3(kBlock), 0, s, logits, c.ld, c.mask, c.rows, c.E,
-                     c.top_k, part_p, part_c, part_n);
+  hipLaunchKernelGGL((balance_fwd_kernel<T, G, C>), dim3(parts), dim3(kThreads), 0, s, logits, c.ld, c.mask, c.rows,
+                     c.E, c.top_k, part_p, part_c, part_n);
   hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(kJoin), 0, s, part_p, part_c, part_n, parts, c.E, c.top_k,
                      c.loss, c.counts, c.kept);
 }
@@ -327,7 +340,7 @@ void launch(const Call &c, int parts, hipStream_t s) {
 int parts_of(int64_t rows, int E, int es) {
   int G, C;
   row_shape(E, 16 / es, &G, &C);
-  const int64_t blocks = ceil_div(rows, kBlock / G);
+  const int64_t blocks = ceil_div(rows, kThreads / G);
   return (int)(blocks < 1 ? 1 : blocks < kMaxParts ? blocks : kMaxParts);
 }
 

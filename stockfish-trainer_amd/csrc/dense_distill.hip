@@ -8,11 +8,13 @@
 // filled slot (or whose teacher logits are all -inf), or without a class above -inf,
 // has loss 0 and no gradient.
 //
-// Bound by reading the logits once and writing the gradient once: a row stays in the
-// registers of the waves that hold it, as loaded, between the maximum, the sum and
-// the gradient.  Rows longer than the registers of a workgroup are read again, from
-// L2 or the memory-side cache.
+// Bound by reading the logits once and writing the gradient once.  A row is read as it
+// comes, with a running maximum and sum per thread, and stays in the registers of the
+// waves that hold it, as loaded, until the gradient; rows longer than a workgroup's
+// registers are read again, from L2 or the memory-side cache.  Rows start anywhere, so
+// chunks are cut where the gradient's (without one: the logits') 16-byte lines are.
 #include "dense.h"
+#include "dense_reduce.h"
 
 namespace sft {
 
@@ -34,30 +36,28 @@ struct Distill {
 
 constexpr int kSlots = SFT_DISTILL_MAX_K / kWave;  // slots per lane
 
-template <int TPR>
-struct Team {  // the threads of a row: a wave, or the workgroup
-  static constexpr int kWaves = TPR / kWave;
-  static __device__ __forceinline__ float max(float x, float *red) {
+// The running maximum m of some x and the sum of 2^((x - m) c).
+struct Running {
+  float m = -INFINITY, sum = 0.f;
+  template <int V>
+  __device__ __forceinline__ void add(const float (&x)[V], float c) {
+    float top = m;
 #pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
-    if (kWaves == 1) return x;
-    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = x;
-    __syncthreads();
-    x = red[0];
+    for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
+    const float at = top == -INFINITY ? 0.f : top;  // nothing above -inf yet: all terms are 0
+    sum *= __builtin_amdgcn_exp2f((m - at) * c);
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) x = fmaxf(x, red[i]);
-    return x;
+    for (int i = 0; i < V; ++i) sum += __builtin_amdgcn_exp2f((x[i] - at) * c);
+    m = top;
   }
-  static __device__ __forceinline__ float sum(float x, float *red) {
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) x += __shfl_xor(x, m);
-    if (kWaves == 1) return x;
-    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = x;
-    __syncthreads();
-    x = red[0];
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) x += red[i];
-    return x;
+  __device__ __forceinline__ float scaled(float top, float c) const {
+    return sum * __builtin_amdgcn_exp2f((m - (top == -INFINITY ? 0.f : top)) * c);
+  }
+  // Over the wave.
+  __device__ __forceinline__ void join(float c) {
+    const float top = dense::group_max<kWave>(m);
+    sum = dense::group_sum<kWave>(scaled(top, c));
+    m = top;
   }
 };
 
@@ -96,11 +96,7 @@ struct Teacher {
       }
       m = t[j] > m || t[j] != t[j] ? t[j] : m;  // a NaN stays
     }
-#pragma unroll
-    for (int x = 1; x < kWave; x <<= 1) {
-      const float o = __shfl_xor(m, x);
-      m = o > m || o != o ? o : m;
-    }
+    m = dense::group_reduce<kWave>(m, [](float a, float b) { return b > a || b != b ? b : a; });
     any = !(m == -INFINITY);
     float sum = 0.f;
 #pragma unroll
@@ -110,8 +106,7 @@ struct Teacher {
       q[j] = any ? expf(t[j] - m) : 0.f;
       sum += q[j];
     }
-#pragma unroll
-    for (int x = 1; x < kWave; x <<= 1) sum += __shfl_xor(sum, x);
+    sum = dense::group_sum<kWave>(sum);
     const float inv = any ? 1.f / sum : 0.f, log_sum = any ? logf(sum) : 0.f;
     cross = 0.f;
 #pragma unroll
@@ -120,8 +115,7 @@ struct Teacher {
       q[j] *= inv;
       if (q[j] != 0.f) cross += q[j] * (t[j] - m - log_sum - at[j]);
     }
-#pragma unroll
-    for (int x = 1; x < kWave; x <<= 1) cross += __shfl_xor(cross, x);
+    cross = dense::group_sum<kWave>(cross);
   }
   // q of the class of slot j, over all its slots (classes may be named twice).
   __device__ __forceinline__ void merged(int k, float (&total)[kSlots]) const {
@@ -140,15 +134,17 @@ struct Teacher {
   }
 };
 
+// The chunk of V elements of a row of n whose first is number `at` (it may hang over
+// either end); -inf outside the row.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T *p, int cnt, u32x4 &v) {
+__device__ __forceinline__ void load_chunk(const T *row, int at, int n, u32x4 &v) {
   constexpr int V = 16 / (int)sizeof(T);
-  if (cnt >= V) {
-    __builtin_memcpy(&v, p, 16);
+  if (at >= 0 && at + V <= n) {
+    __builtin_memcpy(&v, row + at, 16);
   } else {
     T e[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = i < cnt ? p[i] : (T)(-INFINITY);
+    for (int i = 0; i < V; ++i) e[i] = at + i >= 0 && at + i < n ? row[at + i] : (T)(-INFINITY);
     __builtin_memcpy(&v, e, 16);
   }
 }
@@ -160,17 +156,17 @@ __device__ __forceinline__ void unpack(const u32x4 &v, float (&x)[16 / sizeof(T)
   for (int i = 0; i < 16 / (int)sizeof(T); ++i) x[i] = (float)e[i];
 }
 template <typename T>
-__device__ __forceinline__ void store_chunk(T *p, int cnt, const float (&x)[16 / sizeof(T)]) {
+__device__ __forceinline__ void store_chunk(T *row, int at, int n, const float (&x)[16 / sizeof(T)]) {
   constexpr int V = 16 / (int)sizeof(T);
   T e[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) e[i] = (T)x[i];
-  if (cnt >= V) {
-    __builtin_memcpy(p, e, 16);
+  if (at >= 0 && at + V <= n) {
+    __builtin_memcpy(row + at, e, 16);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < cnt) p[i] = e[i];
+      if (at + i >= 0 && at + i < n) row[at + i] = e[i];
   }
 }
 
@@ -178,93 +174,93 @@ __device__ __forceinline__ void store_chunk(T *p, int cnt, const float (&x)[16 /
 // C = 0: the row does not fit, its chunks are read again.
 template <typename T, int TPR, int C>
 __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(const Distill d) {
-  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int V = 16 / (int)sizeof(T), kWaves = TPR / kWave;
   constexpr int kRowsPer = TPR == kWave ? kWavesPerBlock : 1;
-  __shared__ float red[2][TPR / kWave];
-  const int tid = threadIdx.x % TPR;
+  __shared__ float top[kWaves], sums[kWaves];
+  __shared__ float shared_cross;
+  __shared__ int shared_any;
+  const int tid = threadIdx.x % TPR, wave = uniform(tid / kWave);
   const int64_t row = (int64_t)blockIdx.x * kRowsPer + uniform(threadIdx.x / TPR);
-  if (row >= d.rows) return;  // whole waves, and never part of a team
+  if (row >= d.rows) return;  // whole waves, and never part of a row's
   const T *s = static_cast<const T *>(d.s) + row * d.lds;
-  const int chunks = (d.V + V - 1) / V;
-  const bool first = uniform(threadIdx.x / kWave) % (TPR / kWave) == 0;  // the team's first wave
+  T *ds = static_cast<T *>(d.ds) + row * (int64_t)d.V;
+  // chunk c holds the elements from c V - shift on
+  const int shift = (int)((uintptr_t)(d.ds ? ds : s) / sizeof(T) % V);
+  const int chunks = (d.V + shift + V - 1) / V;
+  const float c2 = 1.44269504088896341f / d.tau;  // exp(x / tau) = 2^(x c2)
 
   u32x4 raw[C ? C : 1];
-  float m = -INFINITY;
   if (C) {
 #pragma unroll
-    for (int j = 0; j < C; ++j) load_chunk<T>(s + (int64_t)(tid + TPR * j) * V, d.V - (tid + TPR * j) * V, raw[j]);
+    for (int j = 0; j < C; ++j) load_chunk<T>(s, (tid + TPR * j) * V - shift, d.V, raw[j]);
   }
   Teacher te;
-  te.load(d, row, s);  // every wave: all need `any`
+  if (wave == 0) te.load(d, row, s);
+  Running run;
   if (C) {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       float x[V];
       unpack<T>(raw[j], x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
+      run.add(x, c2);
     }
   } else {
     for (int c = tid; c < chunks; c += TPR) {
       u32x4 v;
       float x[V];
-      load_chunk<T>(s + (int64_t)c * V, d.V - c * V, v);
+      load_chunk<T>(s, c * V - shift, d.V, v);
       unpack<T>(v, x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
+      run.add(x, c2);
     }
   }
-  m = Team<TPR>::max(m, red[0]);
+  run.join(c2);
+  if (kWaves > 1) {
+    if (tid % kWave == 0) {
+      top[wave] = run.m;
+      sums[wave] = run.sum;
+    }
+    if (tid == 0) {
+      shared_cross = te.cross;
+      shared_any = te.any;
+    }
+    __syncthreads();
+    // every wave joins the waves' results, in the same order
+    const int l = lane_id();
+    run.m = l < kWaves ? top[l] : -INFINITY;
+    run.sum = l < kWaves ? sums[l] : 0.f;
+    run.join(c2);
+    te.cross = shared_cross;
+    te.any = shared_any;
+  }
+  const float m = run.m, sum = run.sum;
   const bool live = te.any && m > -INFINITY;
-  const float c2 = 1.44269504088896341f / d.tau;  // exp(x / tau) = 2^(x c2)
-  float sum = 0.f;
-  if (C) {
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      float x[V];
-      unpack<T>(raw[j], x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum += __builtin_amdgcn_exp2f((x[i] - m) * c2);
-    }
-  } else {
-    for (int c = tid; c < chunks; c += TPR) {
-      u32x4 v;
-      float x[V];
-      load_chunk<T>(s + (int64_t)c * V, d.V - c * V, v);
-      unpack<T>(v, x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum += __builtin_amdgcn_exp2f((x[i] - m) * c2);
-    }
-  }
-  sum = Team<TPR>::sum(sum, red[1]);
   if (d.loss && tid == 0) d.loss[row] = live ? d.tau * d.tau * (te.cross + m / d.tau + logf(sum)) : 0.f;
   if (!d.ds) return;
 
-  T *ds = static_cast<T *>(d.ds) + row * (int64_t)d.V;
   const float g = d.tau * (d.weight ? d.weight[row] : 1.f), gp = g / sum;
   auto put = [&](int c, const u32x4 &v) {
     float x[V];
     unpack<T>(v, x);
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] = live ? gp * __builtin_amdgcn_exp2f((x[i] - m) * c2) : 0.f;
-    store_chunk<T>(ds + (int64_t)c * V, d.V - c * V, x);
+    store_chunk<T>(ds, c * V - shift, d.V, x);
   };
   if (C) {
 #pragma unroll
     for (int j = 0; j < C; ++j)
-      if ((tid + TPR * j) * V < d.V) put(tid + TPR * j, raw[j]);
+      if (tid + TPR * j < chunks) put(tid + TPR * j, raw[j]);
   } else {
     for (int c = tid; c < chunks; c += TPR) {
       u32x4 v;
-      load_chunk<T>(s + (int64_t)c * V, d.V - c * V, v);
+      load_chunk<T>(s, c * V - shift, d.V, v);
       put(c, v);
     }
   }
-  if (!live) return;  // the same in the whole team
+  if (!live) return;  // the same for the whole row
   // The teacher's classes once more, after the stores above have been made.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  if (TPR > kWave) __syncthreads();
-  if (!first) return;
+  if (kWaves > 1) __syncthreads();
+  if (wave != 0) return;
   float total[kSlots];
   te.merged(d.k, total);
 #pragma unroll
@@ -276,7 +272,9 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
 template <typename T>
 void launch(const Distill &d, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
-  const int64_t chunks = ceil_div(d.V, V);
+  // rows may start inside a chunk
+  const bool whole = ((uintptr_t)(d.ds ? d.ds : d.s) % 16 | (uintptr_t)((d.ds ? d.V : d.lds) % V)) == 0;
+  const int64_t chunks = ceil_div(d.V, V) + !whole;
 #define SFT_DISTILL(most, TPR, C)                                                                                  \
   if (chunks <= most) {                                                                                            \
     hipLaunchKernelGGL((distill_kernel<T, TPR, C>),                                                                \

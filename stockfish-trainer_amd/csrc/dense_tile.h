@@ -26,37 +26,50 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 #define SFT_LDS __attribute__((address_space(3)))
 
-constexpr int kStageBytes = 128;  // bytes of k per tile row and pipeline stage
+constexpr int kStageBytes = 64;  // bytes of k per tile row and pipeline stage: one fragment's
 
 // ---- activations ----
-// act(z) and its derivative, in binary32.  The derivatives at the kinks are those
-// of torch's clamp: 0 at relu's 0, 1 at both ends of the clipped ones.
-__device__ __forceinline__ float act_value(float z, int act, float &d) {
+// z = act(z) and d = act'(z) of V values, in binary32.  The derivatives at the kinks
+// are those of torch's clamp: 0 at relu's 0, 1 at both ends of the clipped ones.
+template <int V>
+__device__ __forceinline__ void activate(float (&z)[V], float (&d)[V], int act) {
   switch (act) {
     case SFT_ACT_RELU:
-      d = z > 0.f ? 1.f : 0.f;
-      return z < 0.f ? 0.f : z;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        d[i] = z[i] > 0.f ? 1.f : 0.f;
+        z[i] = z[i] < 0.f ? 0.f : z[i];
+      }
+      break;
     case SFT_ACT_CRELU:
-      d = (z >= 0.f && z <= 1.f) ? 1.f : 0.f;
-      return z < 0.f ? 0.f : (z > 1.f ? 1.f : z);
-    case SFT_ACT_SCRELU: {
-      const float c = z < 0.f ? 0.f : (z > 1.f ? 1.f : z);
-      d = (z >= 0.f && z <= 1.f) ? 2.f * c : 0.f;
-      return c * c;
-    }
-    case SFT_ACT_SILU: {
-      const float s = 1.f / (1.f + expf(-z));
-      d = s * (1.f + z * (1.f - s));
-      return z * s;
-    }
-    case SFT_ACT_GELU: {
-      const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-      d = cdf + z * (0.39894228040143268f * expf(-0.5f * z * z));
-      return z * cdf;
-    }
+    case SFT_ACT_SCRELU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float c = z[i] < 0.f ? 0.f : (z[i] > 1.f ? 1.f : z[i]);
+        const float in = (z[i] >= 0.f && z[i] <= 1.f) ? 1.f : 0.f;
+        d[i] = act == SFT_ACT_CRELU ? in : 2.f * c * in;
+        z[i] = act == SFT_ACT_CRELU ? c : c * c;
+      }
+      break;
+    case SFT_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float s = 1.f / (1.f + expf(-z[i]));
+        d[i] = s * (1.f + z[i] * (1.f - s));
+        z[i] *= s;
+      }
+      break;
+    case SFT_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float cdf = 0.5f * (1.f + erff(z[i] * 0.70710678118654752f));
+        d[i] = cdf + z[i] * (0.39894228040143268f * expf(-0.5f * z[i] * z[i]));
+        z[i] *= cdf;
+      }
+      break;
     default:
-      d = 1.f;
-      return z;
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = 1.f;
   }
 }
 
@@ -79,77 +92,64 @@ struct Deriv<float> {
   static __device__ __forceinline__ float unpack(float d) { return d; }
 };
 
-// 4 consecutive elements (guarded: the first `cnt` of them).
-template <typename T>
-struct Quad {
-  T v[4];
-};
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, bool vec, int cnt, T (&v)[4]) {
+// V consecutive elements: in one access, or element by element the first `cnt`.
+template <typename T, int V>
+__device__ __forceinline__ void load_v(const T *p, bool vec, int cnt, T (&v)[V]) {
   if (vec) {
-    const Quad<T> q = *reinterpret_cast<const Quad<T> *>(__builtin_assume_aligned(p, sizeof(T) * 4));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = q.v[i];
+    __builtin_memcpy(v, __builtin_assume_aligned(p, sizeof(T) * V), sizeof(T) * V);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < cnt ? p[i] : (T)0;
+    for (int i = 0; i < V; ++i) v[i] = i < cnt ? p[i] : (T)0;
   }
 }
-template <typename T>
-__device__ __forceinline__ void store4(T *p, bool vec, int cnt, const T (&v)[4]) {
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T *p, bool vec, int cnt, const T (&v)[V]) {
   if (vec) {
-    Quad<T> q;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = v[i];
-    *reinterpret_cast<Quad<T> *>(__builtin_assume_aligned(p, sizeof(T) * 4)) = q;
+    __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T) * V), v, sizeof(T) * V);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < V; ++i)
       if (i < cnt) p[i] = v[i];
   }
 }
 
-// y[m, n..n+3] = residual + act(acc + bias), rounded once; the derivative beside it.
+// y[m, n..n+V-1] = residual + act(z + bias), rounded once; the derivative beside it.
 // Called only with m < M and n < N.
-template <typename T>
-__device__ __forceinline__ void finish4(const Epilogue &e, int64_t m, int n, int N, f32x4 acc) {
+template <typename T, int V>
+__device__ __forceinline__ void finish(const Epilogue &e, int64_t m, int n, int N, float (&z)[V]) {
   const int cnt = N - n;
-  float z[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) z[i] = acc[i];
   if (e.bias) {
-    T b[4];
-    load4(static_cast<const T *>(e.bias) + n, e.vec, cnt, b);
+    T b[V];
+    load_v(static_cast<const T *>(e.bias) + n, e.vec, cnt, b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] += (float)b[i];
+    for (int i = 0; i < V; ++i) z[i] += (float)b[i];
   }
   if (e.act != SFT_ACT_NONE) {
-    float d[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = act_value(z[i], e.act, d[i]);
+    float d[V];
+    activate(z, d, e.act);
     if (e.deriv) {
       typedef typename Deriv<T>::type D;
-      D q[4];
+      D q[V];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = Deriv<T>::pack(d[i]);
-      store4(static_cast<D *>(e.deriv) + m * N + n, e.vec, cnt, q);
+      for (int i = 0; i < V; ++i) q[i] = Deriv<T>::pack(d[i]);
+      store_v(static_cast<D *>(e.deriv) + m * N + n, e.vec, cnt, q);
     }
   }
   if (e.residual) {
-    T r[4];
-    load4(static_cast<const T *>(e.residual) + m * e.ldr + n, e.vec, cnt, r);
+    T r[V];
+    load_v(static_cast<const T *>(e.residual) + m * e.ldr + n, e.vec, cnt, r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] += (float)r[i];
+    for (int i = 0; i < V; ++i) z[i] += (float)r[i];
   }
-  T y[4];
+  T y[V];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = (T)z[i];
-  store4(static_cast<T *>(e.y) + m * e.ldy + n, e.vec, cnt, y);
+  for (int i = 0; i < V; ++i) y[i] = (T)z[i];
+  store_v(static_cast<T *>(e.y) + m * e.ldy + n, e.vec, cnt, y);
 }
 
 // ---- tiles in LDS ----
 // A stage of an operand is kStageBytes of k for each of its BMN rows (m or n), held
-// in 16-byte chunks.  k-major: [BMN][128 bytes]; row-k: [stage k][BMN].  Chunks are
+// in 16-byte chunks.  k-major: [BMN][64 bytes]; row-k: [stage k][BMN].  Chunks are
 // permuted within a row so that the reads below touch every LDS bank equally; the
 // copies from global memory write LDS linearly (the hardware's rule for direct
 // copies: lane l writes base + 16 l), so the permutation is applied to the global
@@ -164,14 +164,14 @@ struct TileMap {
   static constexpr int kBytes = BMN * kStageBytes;
   // The chunk of its row that the slot holds.
   static __device__ __forceinline__ int chunk_at(int row, int slot) {
-    if (KMAJ) return slot ^ ((row >> 1) & 7);
+    if (KMAJ) return slot ^ ((0 - (row >> 2)) & 3);
     if (kEs == 2) return slot ^ (((((row & 3) | ((row >> 1) & 4)) << 1)) & (kRowChunks - 1));
     return slot ^ ((((row >> 2) & 3) << 2) & (kRowChunks - 1));
   }
 };
 
 // Copies a stage's chunks straight to LDS with bounds-checked buffer loads (out of
-// range reads give zeros).  Needs 16-byte aligned rows and whole chunks.
+// range reads give zeros).  Rows are 16-byte aligned and hold whole chunks.
 template <typename T, int BMN, bool KMAJ, int THREADS>
 struct DirectLoader {
   typedef TileMap<T, BMN, KMAJ> Map;
@@ -201,13 +201,13 @@ struct DirectLoader {
       const int row = q / Map::kRowChunks, c = Map::chunk_at(row, q % Map::kRowChunks);
       off[j] = (uint32_t)row * (uint32_t)(ld * Map::kEs) + (uint32_t)c * 16u;
       if (!KMAJ && mn0 + c * Map::kEpc >= MN) off[j] = kOut;
-      if (KMAJ) kchunk = c * Map::kEpc;  // the same for every j: THREADS / 8 rows apart
+      if (KMAJ) kchunk = c * Map::kEpc;  // the same for every j: THREADS / 4 rows apart
     }
   }
   // kleft: k from the stage's first to the end of the range.
-  __device__ __forceinline__ void load(char *lds, int kleft) {
+  __device__ __forceinline__ void load(SFT_LDS char *lds, int kleft) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass has no such builtins
-    const uint32_t n = (uint32_t)(left < 0x7ffffff0ll ? left : 0x7ffffff0ll);
+    const uint32_t n = left <= 0 ? 0u : (uint32_t)(left < 0x7ffffff0ll ? left : 0x7ffffff0ll);
     const __amdgpu_buffer_rsrc_t r =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)n, 0x00020000);
     const int wave = uniform(threadIdx.x / kWave);
@@ -220,52 +220,24 @@ struct DirectLoader {
     base += step;
     left -= step;
   }
-  __device__ __forceinline__ void store(char *) {}
 };
 
-// The same stage through registers, for any alignment and size: a chunk is read
-// whole where it lies inside the operand, element by element at its edge.
-template <typename T, int BMN, bool KMAJ, int THREADS>
-struct GuardedLoader {
-  typedef TileMap<T, BMN, KMAJ> Map;
-  static constexpr int kLoads = Map::kBytes / 16 / THREADS;
-  const T *base;
-  int64_t ld;
-  int mnleft;  // rows of the operand from the tile's first
-  u32x4 v[kLoads];
-  __device__ __forceinline__ void init(const void *p, int64_t ld_, int mn0, int MN, int k0, int) {
-    ld = ld_;
-    mnleft = MN - mn0;
-    base = static_cast<const T *>(p) + (KMAJ ? (int64_t)mn0 * ld + k0 : (int64_t)k0 * ld + mn0);
-  }
-  __device__ __forceinline__ void load(char *, int kleft) {
+// A 16-byte chunk whose first `cnt` elements exist; zeros after them.  The hardware
+// takes any element alignment.
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T *p, int64_t cnt) {
+  constexpr int V = 16 / (int)sizeof(T);
+  u32x4 r = {0u, 0u, 0u, 0u};
+  if (cnt >= V) {
+    __builtin_memcpy(&r, p, 16);
+  } else if (cnt > 0) {
+    T e[V];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int q = j * THREADS + threadIdx.x;
-      const int row = q / Map::kRowChunks, c = Map::chunk_at(row, q % Map::kRowChunks) * Map::kEpc;
-      const int rows = KMAJ ? mnleft : kleft, cols = KMAJ ? kleft : mnleft;
-      v[j] = load_chunk<T>(base + row * ld + c, row < rows ? cols - c : 0);
-    }
-    base += KMAJ ? Map::kStageK : Map::kStageK * ld;
+    for (int i = 0; i < V; ++i) e[i] = i < cnt ? p[i] : (T)0;
+    __builtin_memcpy(&r, e, 16);
   }
-  __device__ __forceinline__ void store(char *lds) {
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4 *>(lds + (j * THREADS + threadIdx.x) * 16) = v[j];
-  }
-  template <typename U>
-  static __device__ __forceinline__ u32x4 load_chunk(const U *p, int cnt) {
-    u32x4 r = {0u, 0u, 0u, 0u};
-    if (cnt >= 16 / (int)sizeof(U)) {
-      __builtin_memcpy(&r, p, 16);  // one 16-byte load: the hardware takes any element alignment
-    } else if (cnt > 0) {
-      U e[16 / sizeof(U)];
-#pragma unroll
-      for (int i = 0; i < 16 / (int)sizeof(U); ++i) e[i] = i < cnt ? p[i] : (U)0;
-      __builtin_memcpy(&r, e, 16);
-    }
-    return r;
-  }
-};
+  return r;
+}
 
 // ---- fragments: 16 rows (m or n) by 64 bytes of k, as the matrix instructions take them ----
 template <typename T>
@@ -282,39 +254,55 @@ template <>
 struct Frag<float> {
   u32x4 v;  // four k of one row
 };
+// One step of a fragment's k: all 64 bytes of 16-bit types, a quarter of binary32's.
 template <typename T>
-__device__ __forceinline__ f32x4 mma(const Frag<T> &a, const Frag<T> &b, f32x4 c);
+struct Mma;
 template <>
-__device__ __forceinline__ f32x4 mma(const Frag<bf16_t> &a, const Frag<bf16_t> &b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), c,
-                                                 0, 0, 0);
-}
+struct Mma<bf16_t> {
+  static constexpr int kSteps = 1;
+  static __device__ __forceinline__ f32x4 step(const Frag<bf16_t> &a, const Frag<bf16_t> &b, f32x4 c, int) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v),
+                                                   c, 0, 0, 0);
+  }
+};
 template <>
-__device__ __forceinline__ f32x4 mma(const Frag<f16_t> &a, const Frag<f16_t> &b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v), __builtin_bit_cast(f16x8, b.v), c, 0,
-                                                0, 0);
-}
+struct Mma<f16_t> {
+  static constexpr int kSteps = 1;
+  static __device__ __forceinline__ f32x4 step(const Frag<f16_t> &a, const Frag<f16_t> &b, f32x4 c, int) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v), __builtin_bit_cast(f16x8, b.v), c,
+                                                  0, 0, 0);
+  }
+};
 template <>
-__device__ __forceinline__ f32x4 mma(const Frag<float> &a, const Frag<float> &b, f32x4 c) {
-  const f32x4 fa = __builtin_bit_cast(f32x4, a.v), fb = __builtin_bit_cast(f32x4, b.v);
+struct Mma<float> {
+  static constexpr int kSteps = 4;
+  static __device__ __forceinline__ f32x4 step(const Frag<float> &a, const Frag<float> &b, f32x4 c, int s) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, a.v)[s], __builtin_bit_cast(f32x4, b.v)[s],
+                                                c, 0, 0, 0);
+  }
+};
+// acc[i][j] += the product of fragment i of A and j < NJ of B.
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void mma_all(const Frag<T> (&fa)[FM], const Frag<T> (&fb)[FN], f32x4 (&acc)[FM][FN]) {
 #pragma unroll
-  for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[s], fb[s], c, 0, 0, 0);
-  return c;
+  for (int s = 0; s < Mma<T>::kSteps; ++s)
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::step(fb[j], fa[i], acc[i][j], s);
 }
 
-// Reads fragments of F consecutive 16-row groups of an LDS tile, from row mn0.
-// Lane l holds row l % 16, and of each 64 bytes of k the 16 bytes number l / 16.
+// Reads the fragments of F consecutive 16-row groups of an LDS tile, from row mn0.
+// Lane l holds row l % 16 and the 16 bytes number l / 16 of its 64 bytes of k.
 template <typename T, int BMN, bool KMAJ, int F>
 struct FragReader {
   typedef TileMap<T, BMN, KMAJ> Map;
-  int at[KMAJ ? 2 : F];
+  int at[KMAJ ? 1 : F];
   __device__ __forceinline__ void init(int mn0) {
     const int i = lane_id() % 16, g = lane_id() / 16;
     if (KMAJ) {
-      const int row = mn0 + i;
-      // mn0 + 16 f leaves the permutation as it is
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) at[kk] = row * kStageBytes + (Map::chunk_at(row, kk * 4 + g) << 4);
+      const int row = mn0 + i;  // 16 f more rows leave the permutation as it is
+      at[0] = row * kStageBytes + (Map::chunk_at(row, g) << 4);
     } else if (Map::kEs == 2) {
       // A transposing read gives lane i of 16 the element i of 4 rows: the lane reads
       // 4 elements of row i / 4 and gets one of each row.
@@ -329,20 +317,20 @@ struct FragReader {
         at[f] = row * Map::kRowBytes + (Map::chunk_at(row, (mn0 / 16 + f) * 4 + i / 4) << 4) + (i % 4) * 4;
     }
   }
-  __device__ __forceinline__ Frag<T> read(const char *lds, int f, int kk) const {
+  __device__ __forceinline__ Frag<T> read(const SFT_LDS char *lds, int f) const {
     Frag<T> r;
     if constexpr (KMAJ) {
-      r.v = *reinterpret_cast<const u32x4 *>(lds + at[kk] + f * 16 * kStageBytes);
+      r.v = *(const SFT_LDS u32x4 *)(lds + at[0] + f * 16 * kStageBytes);
     } else if constexpr (Map::kEs == 2) {
-      const char *p = lds + at[f] + kk * 32 * Map::kRowBytes;
+      const SFT_LDS char *p = lds + at[f];
       const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((SFT_LDS i16x4 *)p));
       const u32x2 hi = __builtin_bit_cast(
           u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((SFT_LDS i16x4 *)(p + 4 * Map::kRowBytes)));
       r.v = u32x4{lo.x, lo.y, hi.x, hi.y};
     } else {
-      const char *p = lds + at[f] + kk * 16 * Map::kRowBytes;
+      const SFT_LDS char *p = lds + at[f];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) r.v[s] = *reinterpret_cast<const uint32_t *>(p + s * Map::kRowBytes);
+      for (int s = 0; s < 4; ++s) r.v[s] = *(const SFT_LDS uint32_t *)(p + s * Map::kRowBytes);
     }
     return r;
   }
@@ -367,113 +355,184 @@ __device__ __forceinline__ void tile_of(const Gemm &g, int &tm, int &tn, int &sp
   tn = (int)(in / rows);
 }
 
-// BM x BN outputs per workgroup of WM x WN waves; two LDS stages, the copy of one
-// beside the products of the other.
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, bool DIRECT>
-__global__ __launch_bounds__(WM *WN *kWave) void gemm_tile_kernel(const Gemm g) {
-  constexpr int kThreads = WM * WN * kWave;
-  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int kStageK = kStageBytes / (int)sizeof(T);
-  constexpr int kStage = (BM + BN) * kStageBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
-  int tm, tn, split;
-  tile_of(g, tm, tn, split);
-  const int m0 = tm * BM, n0 = tn * BN;
-  const int k0 = split * g.split_k;
-  const int kend = g.K - k0 < g.split_k ? g.K : k0 + g.split_k;
-  const int wave = uniform(threadIdx.x / kWave);
-  const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+// What a workgroup of WM x WN waves does with its BM x BN sums.
+template <typename T, int BM, int BN, int WM, int WN>
+struct TileWork {
+  static constexpr int kThreads = WM * WN * kWave;
+  static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+  static constexpr int kStageK = kStageBytes / (int)sizeof(T);
+  static constexpr int kStage = (BM + BN) * kStageBytes;
+  int split, m0, n0, wm, wn, k0, kend;
+  __device__ __forceinline__ explicit TileWork(const Gemm &g) {
+    int tm, tn;
+    tile_of(g, tm, tn, split);
+    m0 = tm * BM;
+    n0 = tn * BN;
+    k0 = split * g.split_k;
+    kend = g.K - k0 < g.split_k ? g.K : k0 + g.split_k;
+    const int wave = uniform(threadIdx.x / kWave);
+    wm = (wave / WN) * (BM / WM);
+    wn = (wave % WN) * (BN / WN);
+  }
+  // The first operand's rows are the result's four registers: lane l holds m = l % 16
+  // and n = 4 (l / 16) + 0..3 of each fragment.  A wave turns its sums in LDS, a part
+  // of the rows at a time, so that its lanes take whole vectors of a row: memory sees
+  // full lines, and the epilogue's code is there once per part.
+  static constexpr int kWaveN = BN / WN, kPitch = kWaveN + 4;  // floats; 4 spread the rows over the banks
+  static constexpr int kParts = FM / 2;  // 32 rows
+  static constexpr int kPartM = FM / kParts;
+  static constexpr int kTurnBytes = kPartM * 16 * kPitch * 4 * WM * WN;
+  __device__ __forceinline__ void finish_all(const Gemm &g, const f32x4 (&acc)[FM][FN], char *lds) const {
+    constexpr int V = 16 / (int)sizeof(T), kLanes = kWaveN / V, kRows = kWave / kLanes;
+    const int lane = lane_id();
+    float *turn = reinterpret_cast<float *>(lds) + (threadIdx.x / kWave) * (kPartM * 16 * kPitch);
+    const int n = n0 + wn + lane % kLanes * V;
+    __syncthreads();  // every wave has done with the stages
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+      for (int i = 0; i < kPartM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          *reinterpret_cast<f32x4 *>(turn + (i * 16 + lane % 16) * kPitch + j * 16 + lane / 16 * 4) =
+              acc[part * kPartM + i][j];
+      wave_lds_barrier();
+#pragma unroll 1
+      for (int r = lane / kLanes; r < kPartM * 16; r += kRows) {
+        const int m = m0 + wm + part * kPartM * 16 + r;
+        if (m >= g.M || n >= g.N) break;
+        float z[V];
+#pragma unroll
+        for (int i = 0; i < V; i += 4)
+          *reinterpret_cast<f32x4 *>(z + i) =
+              *reinterpret_cast<const f32x4 *>(turn + r * kPitch + lane % kLanes * V + i);
+        if (g.part)
+          store_v(g.part + ((int64_t)split * g.M + m) * g.N + n, g.N % V == 0, g.N - n, z);
+        else
+          finish<T>(g.epi, m, n, g.N, z);
+      }
+      wave_lds_barrier();
+    }
+  }
+};
 
-  typedef typename std::conditional<DIRECT, DirectLoader<T, BM, AK, kThreads>,
-                                    GuardedLoader<T, BM, AK, kThreads>>::type LoadA;
-  typedef typename std::conditional<DIRECT, DirectLoader<T, BN, BK, kThreads>,
-                                    GuardedLoader<T, BN, BK, kThreads>>::type LoadB;
+// Aligned operands.  Three things overlap: the copies of stages s + 2 .. s + RING
+// from memory to a ring in LDS, the reads of stage s + 1's fragments into registers,
+// and the products of stage s.  The copies carry their own bounds checks, so those
+// past the end are made too (they give zeros) and every stage waits for the same
+// number of outstanding ones.
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int RING>
+__global__ __launch_bounds__(WM *WN *kWave, BM / WM * BN / WN > 128 * 64 ? 1 : 2) void gemm_ring_kernel(const Gemm g) {
+  typedef TileWork<T, BM, BN, WM, WN> Work;
+  constexpr int FM = Work::FM, FN = Work::FN, kStage = Work::kStage;
+  typedef DirectLoader<T, BM, AK, Work::kThreads> LoadA;
+  typedef DirectLoader<T, BN, BK, Work::kThreads> LoadB;
+  constexpr int kCopies = LoadA::kLoads + LoadB::kLoads;
+  __shared__ __attribute__((aligned(1024))) char lds[RING * kStage > Work::kTurnBytes ? RING * kStage
+                                                                                   : Work::kTurnBytes];
+  const Work w(g);
   LoadA la;
   LoadB lb;
-  la.init(g.a, g.lda, m0, g.M, k0, kend);
-  lb.init(g.b, g.ldb, n0, g.N, k0, kend);
+  la.init(g.a, g.lda, w.m0, g.ma, w.k0, w.kend < g.ka ? w.kend : g.ka);
+  lb.init(g.b, g.ldb, w.n0, g.nb, w.k0, w.kend < g.kb ? w.kend : g.kb);
   FragReader<T, BM, AK, FM> ra;
   FragReader<T, BN, BK, FN> rb;
-  ra.init(wm);
-  rb.init(wn);
-
-  f32x4 acc[FM][FN];
+  ra.init(w.wm);
+  rb.init(w.wn);
+  f32x4 acc[FM][FN] = {};
+  int kleft = w.kend - w.k0;
+  const int steps = (kleft + Work::kStageK - 1) / Work::kStageK;
+  SFT_LDS char *ring = (SFT_LDS char *)lds;
+  // The two slots of one call differ; without the restricts the compiler would wait
+  // for the copies before it reads.
+  auto copy = [&](SFT_LDS char *__restrict__ to) {
+    la.load(to, kleft);
+    lb.load(to + BM * kStageBytes, kleft);
+    kleft -= Work::kStageK;
+  };
+  auto copy_read = [&](SFT_LDS char *__restrict__ to, const SFT_LDS char *__restrict__ from, Frag<T>(&fa)[FM],
+                       Frag<T>(&fb)[FN]) {
+    la.load(to, kleft);
+    lb.load(to + BM * kStageBytes, kleft);
+    kleft -= Work::kStageK;
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+    for (int i = 0; i < FM; ++i) fa[i] = ra.read(from, i);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const int steps = (kend - k0 + kStageK - 1) / kStageK;
-  la.load(lds, kend - k0);
-  lb.load(lds + BM * kStageBytes, kend - k0);
-  la.store(lds);
-  lb.store(lds + BM * kStageBytes);
-  for (int it = 0; it < steps; ++it) {
-    char *cur = lds + (it & 1) * kStage, *nxt = lds + (~it & 1) * kStage;
-    // this stage has arrived, and every wave has done with the other one
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const bool more = it + 1 < steps;
-    if (more) {
-      const int kleft = kend - k0 - (it + 1) * kStageK;
-      la.load(nxt, kleft);
-      lb.load(nxt + BM * kStageBytes, kleft);
+    for (int j = 0; j < FN; ++j) fb[j] = rb.read(from + BM * kStageBytes, j);
+  };
+  // Own copies up to the last RING - 2 stages' are in LDS and own fragment reads are
+  // done; then the same holds for every wave.
+  auto meet = [&]() {
+    constexpr int kLeft = (RING - 2) * kCopies;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((kLeft & 15) | (kLeft >> 4 << 14) | 0x70);  // vmcnt(kLeft) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // The order of one stage: products between the copies and the fragment reads.
+  auto interleave = []() {
+    constexpr int kReads = FM * (AK ? 1 : sizeof(T) == 2 ? 2 : 4) + FN * (BK ? 1 : sizeof(T) == 2 ? 2 : 4);
+    constexpr int kProducts = FM * FN * Mma<T>::kSteps, kGroups = kReads + kCopies;
+    constexpr int kPer = kProducts / kGroups > 0 ? kProducts / kGroups : 1;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // memory read
+      __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);  // matrix instruction
     }
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      Frag<T> fa[FM], fb[FN];
-#pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = ra.read(cur, i, kk);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = rb.read(cur + BM * kStageBytes, j, kk);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(fb[j], fa[i], acc[i][j]);
+    for (int i = 0; i < kReads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
     }
-    if (more) {
-      la.store(nxt);
-      lb.store(nxt + BM * kStageBytes);
-    }
-  }
-  // The first operand's rows are the result's four registers: lane l holds
-  // m = l % 16 and n = 4 (l / 16) + 0..3 of each fragment.
-  const int lane = lane_id();
+    __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+  };
+  for (int s = 0; s < RING - 1; ++s) copy(ring + s * kStage);
+  Frag<T> fa[2][FM], fb[2][FN];
+  meet();  // stage 0
+  copy_read(ring + (RING - 1) * kStage, ring, fa[0], fb[0]);
+  int slot = 1;
+  if (w.m0 + w.wm < g.M && w.n0 + w.wn < g.N) {
+    for (int s = 0; s < steps; s += 2) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = m0 + wm + i * 16 + lane % 16;
-    if (m >= g.M) continue;
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = n0 + wn + j * 16 + lane / 16 * 4;
-      if (n >= g.N) continue;
-      if (g.part) {
-        float v[4] = {acc[i][j].x, acc[i][j].y, acc[i][j].z, acc[i][j].w};
-        store4(g.part + ((int64_t)split * g.M + m) * g.N + n, g.N % 4 == 0, g.N - n, v);
-      } else {
-        finish4<T>(g.epi, m, n, g.N, acc[i][j]);
+      for (int h = 0; h < 2; ++h) {
+        if (s + h < steps) {
+          meet();  // stage s + h + 1 is in LDS, the slot of stage s + h is free
+          copy_read(ring + (slot == 0 ? RING - 1 : slot - 1) * kStage, ring + slot * kStage, fa[1 - h], fb[1 - h]);
+          mma_all<T>(fa[h], fb[h], acc);
+          interleave();
+          slot = slot == RING - 1 ? 0 : slot + 1;
+        }
       }
     }
+  } else {  // a wave past the edge: its share of the copies only
+    for (int s = 0; s < steps; ++s) {
+      meet();
+      copy(ring + (slot == 0 ? RING - 1 : slot - 1) * kStage);
+      slot = slot == RING - 1 ? 0 : slot + 1;
+    }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the stages
+  w.finish_all(g, acc, lds);
 }
 
 // Sums a split product's partials in split order and finishes them.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void gemm_join_kernel(const Gemm g) {
-  const int64_t quads = (g.N + 3) / 4;
+  constexpr int V = 16 / (int)sizeof(T);
+  const int64_t vecs = (g.N + V - 1) / V;
   const int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (q >= quads * g.M) return;
-  const int64_t m = q / quads;
-  const int n = (int)(q % quads) * 4;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (q >= vecs * g.M) return;
+  const int64_t m = q / vecs;
+  const int n = (int)(q % vecs) * V;
+  float z[V] = {};
   const float *p = g.part + m * g.N + n;
   for (int s = 0; s < g.splits; ++s, p += (int64_t)g.M * g.N) {
-    float v[4];
-    load4(p, g.N % 4 == 0, g.N - n, v);
+    float v[V];
+    load_v(p, g.N % V == 0, g.N - n, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += v[i];
+    for (int i = 0; i < V; ++i) z[i] += v[i];
   }
-  finish4<T>(g.epi, m, n, g.N, acc);
+  finish<T>(g.epi, m, n, g.N, z);
 }
 
 // ---- few rows ----
@@ -500,20 +559,21 @@ __global__ __launch_bounds__(kRowWaves *kWave) void gemm_rows_kernel(const Gemm 
   f32x4 acc[FM];
 #pragma unroll
   for (int f = 0; f < FM; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  typedef GuardedLoader<T, 16, true, kWave> Chunk;
   for (int k0 = wave * kPiece; k0 < g.K; k0 += kRowWaves * kPiece) {
     Frag<T> fw[4], fx[FM][4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int k = k0 + (u * 4 + c) * kEpc;
-      fw[u].v = Chunk::load_chunk(w + k, nin ? g.K - k : 0);
+      fw[u].v = load_chunk(w + k, nin ? g.K - k : 0);
 #pragma unroll
-      for (int f = 0; f < FM; ++f) fx[f][u].v = Chunk::load_chunk(x[f] + k, in[f] ? g.K - k : 0);
+      for (int f = 0; f < FM; ++f) fx[f][u].v = load_chunk(x[f] + k, in[f] ? g.K - k : 0);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int f = 0; f < FM; ++f) acc[f] = mma<T>(fw[u], fx[f][u], acc[f]);
+      for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int t = 0; t < Mma<T>::kSteps; ++t) acc[f] = Mma<T>::step(fw[u], fx[f][u], acc[f], t);
   }
 #pragma unroll
   for (int f = 0; f < FM; ++f) red[wave][f][lane] = acc[f];
@@ -524,42 +584,46 @@ __global__ __launch_bounds__(kRowWaves *kWave) void gemm_rows_kernel(const Gemm 
 #pragma unroll
   for (int s = 1; s < kRowWaves; ++s) sum += red[s][f][lane];
   const int m = f * 16 + i, n = n0 + c * 4;
-  if (m < g.M && n < g.N) finish4<T>(g.epi, m, n, g.N, sum);
+  float z[4] = {sum.x, sum.y, sum.z, sum.w};
+  if (m < g.M && n < g.N) finish<T>(g.epi, m, n, g.N, z);
 }
 
 // ---- gradient of the activation, and the bias grad's partial sums ----
-// dz = dy * act'(z), rounded to the layer's type for the products that follow, and
-// the sums of the unrounded dz over `rows` rows per workgroup and column.  A thread
-// holds V columns; a workgroup is tx column groups by 256 / tx rows.
-template <typename T, int V>
+// dz = dy * act'(z), rounded to the layer's type for the products that follow (its
+// rows are padded with zeros to whole chunks), and the sums of the unrounded dz over
+// `rows` rows per workgroup and column.  A thread holds a chunk of V columns; a
+// workgroup is tx chunks by 256 / tx rows.  Reading and writing bound it: 4.6 TB/s at
+// 65536 x 4096.
+template <typename T>
 __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
   typedef typename Deriv<T>::type D;
+  constexpr int V = 16 / (int)sizeof(T);
   __shared__ float red[kBlock * V];
   const int tx = p.tx, ty = kBlock / tx;
   const int cx = threadIdx.x % tx, ry = threadIdx.x / tx;
-  const int n = (blockIdx.x * tx + cx) * V;
+  const int n = (blockIdx.x * tx + cx) * V, cnt = p.N - n;
   const int64_t first = (int64_t)blockIdx.y * p.rows;
   const int64_t last = first + p.rows < p.M ? first + p.rows : p.M;
   float sum[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = 0.f;
-  if (n < p.N) {
+  if (cnt > 0) {
     for (int64_t m = first + ry; m < last; m += ty) {
       T dy[V];
-      __builtin_memcpy(dy, static_cast<const T *>(p.dy) + m * p.lddy + n, sizeof(T) * V);
+      *reinterpret_cast<u32x4 *>(dy) = load_chunk(static_cast<const T *>(p.dy) + m * p.lddy + n, cnt);
       float v[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = (float)dy[i];
       if (p.deriv) {
         D d[V];
-        __builtin_memcpy(d, static_cast<const D *>(p.deriv) + m * p.N + n, sizeof(D) * V);
+        *reinterpret_cast<u32x4 *>(d) = load_chunk(static_cast<const D *>(p.deriv) + m * p.N + n, cnt);
         T dz[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          v[i] *= Deriv<T>::unpack(d[i]);
+          v[i] = i < cnt ? v[i] * Deriv<T>::unpack(d[i]) : 0.f;
           dz[i] = (T)v[i];
         }
-        __builtin_memcpy(static_cast<T *>(p.dz) + m * p.N + n, dz, sizeof(T) * V);
+        *reinterpret_cast<u32x4 *>(static_cast<T *>(p.dz) + m * p.lddz + n) = *reinterpret_cast<u32x4 *>(dz);
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) sum[i] += v[i];
@@ -567,47 +631,68 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
   }
   if (!p.part) return;
 #pragma unroll
-  for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = sum[i];
+  for (int i = 0; i < V; ++i) red[i * kBlock + threadIdx.x] = sum[i];
   __syncthreads();
-  if (ry != 0 || n >= p.N) return;
+  if (ry != 0 || cnt <= 0) return;
   for (int r = 1; r < ty; ++r)
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] += red[(r * tx + cx) * V + i];
+    for (int i = 0; i < V; ++i) sum[i] += red[i * kBlock + r * tx + cx];
 #pragma unroll
-  for (int i = 0; i < V; ++i) p.part[(int64_t)blockIdx.y * p.N + n + i] = sum[i];
+  for (int i = 0; i < V; ++i)
+    if (i < cnt) p.part[(int64_t)blockIdx.y * p.N + n + i] = sum[i];
 }
 
-// db[n] = the partials of column n in order.  A workgroup holds 64 columns, its four
-// waves a quarter of the partials each.
+// db[n] = the sum of column n's partials: 64 threads take every 64th each, and are
+// added in order.
+constexpr int kJoinCols = 16, kJoinRows = 64;
 template <typename T>
-__global__ __launch_bounds__(kBlock) void bias_join_kernel(const float *__restrict__ part, int parts, int N, void *db) {
-  __shared__ float red[kWavesPerBlock][kWave];
-  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-  const int n = blockIdx.x * kWave + lane;
-  const int per = (parts + kWavesPerBlock - 1) / kWavesPerBlock;
+__global__ __launch_bounds__(kJoinCols *kJoinRows) void bias_join_kernel(const float *__restrict__ part, int parts,
+                                                                         int N, void *db) {
+  __shared__ float red[kJoinRows][kJoinCols];
+  const int c = threadIdx.x % kJoinCols, r = threadIdx.x / kJoinCols;
+  const int n = blockIdx.x * kJoinCols + c;
   float s = 0.f;
   if (n < N)
-    for (int r = w * per; r < (w + 1) * per && r < parts; ++r) s += part[(int64_t)r * N + n];
-  red[w][lane] = s;
+    for (int i = r; i < parts; i += kJoinRows) s += part[(int64_t)i * N + n];
+  red[r][c] = s;
   __syncthreads();
-  if (w == 0 && n < N) static_cast<T *>(db)[n] = (T)((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+  if (r != 0 || n >= N) return;
+  for (int i = 1; i < kJoinRows; ++i) s += red[i][c];
+  static_cast<T *>(db)[n] = (T)s;
+}
+
+// ---- copies of operands with whole, aligned rows ----
+// Up to two matrices of rows x cols elements, to rows of a whole number of chunks with
+// zeros past cols.  One chunk a thread.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void align_rows_kernel(const Copy a, const Copy b, int64_t blocks_a) {
+  const bool second = (int64_t)blockIdx.x >= blocks_a;
+  const Copy c = second ? b : a;
+  const int64_t q = ((int64_t)blockIdx.x - (second ? blocks_a : 0)) * kBlock + threadIdx.x;
+  const int64_t chunks = c.to_ld / (16 / (int)sizeof(T)), row = q / chunks, at = q % chunks * (16 / (int)sizeof(T));
+  if (row >= c.rows) return;
+  *reinterpret_cast<u32x4 *>(static_cast<T *>(c.to) + row * c.to_ld + at) =
+      load_chunk(static_cast<const T *>(c.from) + row * c.ld + at, c.cols - at);
 }
 
 // ---- launchers, instantiated per type ----
 template <typename T, bool AK, bool BK>
 int launch_gemm_as(const Gemm &g, hipStream_t s) {
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-#define SFT_TILE(BM, BN, WM, WN, DIRECT)                                                                       \
-  hipLaunchKernelGGL((gemm_tile_kernel<T, AK, BK, BM, BN, WM, WN, DIRECT>), dim3((unsigned)grid),              \
+#define SFT_RING(BM, BN, WM, WN, RING)                                                                  \
+  hipLaunchKernelGGL((gemm_ring_kernel<T, AK, BK, BM, BN, WM, WN, RING>), dim3((unsigned)grid),         \
                      dim3(WM *WN *kWave), 0, s, g)
-  if (g.direct)
-    SFT_TILE(128, 128, 2, 2, true);
-  else
-    SFT_TILE(128, 128, 2, 2, false);
-#undef SFT_TILE
+  if (g.tile == kTile64) {
+    SFT_RING(64, 128, 2, 2, 4);
+  } else if (g.tile == kTile128) {
+    SFT_RING(128, 128, 2, 2, 3);
+  } else {
+    if constexpr (sizeof(T) == 2) SFT_RING(256, 256, 2, 4, 4);
+  }
+#undef SFT_RING
   if (g.splits > 1) {
-    const int64_t quads = ((int64_t)g.N + 3) / 4 * g.M;
-    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)ceil_div(quads, kBlock)), dim3(kBlock), 0, s, g);
+    const int64_t vecs = ceil_div(g.N, 16 / (int64_t)sizeof(T)) * g.M;
+    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)ceil_div(vecs, kBlock)), dim3(kBlock), 0, s, g);
   }
   return check_launch("dense product");
 }
@@ -633,23 +718,28 @@ int launch_rows(const Gemm &g, hipStream_t s) {
 
 template <typename T>
 int launch_act_bwd(const ActBwd &p, void *db, hipStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int cols = p.vec ? (int)ceil_div(p.N, V) : p.N;
-  const dim3 grid((unsigned)ceil_div(cols, p.tx), (unsigned)p.parts);
-  if (p.vec)
-    hipLaunchKernelGGL((act_bwd_kernel<T, V>), grid, dim3(kBlock), 0, s, p);
-  else
-    hipLaunchKernelGGL((act_bwd_kernel<T, 1>), grid, dim3(kBlock), 0, s, p);
+  const int64_t chunks = ceil_div(p.N, 16 / (int64_t)sizeof(T));
+  hipLaunchKernelGGL((act_bwd_kernel<T>), dim3((unsigned)ceil_div(chunks, p.tx), (unsigned)p.parts), dim3(kBlock), 0, s,
+                     p);
   if (db)
-    hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)ceil_div(p.N, kWave)), dim3(kBlock), 0, s, p.part,
-                       p.parts, p.N, db);
+    hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)ceil_div(p.N, kJoinCols)), dim3(kJoinCols * kJoinRows), 0,
+                       s, p.part, p.parts, p.N, db);
   return check_launch("dense activation backward");
+}
+
+template <typename T>
+int launch_align(const Copy &a, const Copy &b, hipStream_t s) {
+  const int64_t epc = 16 / (int64_t)sizeof(T);
+  const int64_t na = ceil_div(a.rows * (a.to_ld / epc), kBlock), nb = ceil_div(b.rows * (b.to_ld / epc), kBlock);
+  hipLaunchKernelGGL((align_rows_kernel<T>), dim3((unsigned)(na + nb)), dim3(kBlock), 0, s, a, b, na);
+  return check_launch("dense aligned copy");
 }
 
 #define SFT_DENSE_TYPE(T)                                                \
   template int launch_gemm<T>(const Gemm &, int, hipStream_t);           \
   template int launch_rows<T>(const Gemm &, hipStream_t);                \
-  template int launch_act_bwd<T>(const ActBwd &, void *, hipStream_t);
+  template int launch_act_bwd<T>(const ActBwd &, void *, hipStream_t);   \
+  template int launch_align<T>(const Copy &, const Copy &, hipStream_t);
 
 }  // namespace dense
 }  // namespace sft

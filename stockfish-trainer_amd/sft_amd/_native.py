@@ -44,6 +44,7 @@ SFT_ACT_CRELU = 2
 SFT_ACT_SCRELU = 3
 SFT_ACT_SILU = 4
 SFT_ACT_GELU = 5
+SFT_LINEAR_COPY = 0x1
 SFT_BALANCE_MAX_EXPERTS = 1024
 SFT_DISTILL_MAX_K = 256
 SFT_FEATURES_THREATS = 1
@@ -124,13 +125,14 @@ SIGNATURES = {
     "sft_leb128_workspace_size": (ctypes.c_int, [_i64, ctypes.POINTER(ctypes.c_size_t)]),
     "sft_leb128_encode": (ctypes.c_int, [_vp, _i32, _i64, _vp, ctypes.c_size_t, _vp, _vp, ctypes.c_size_t, _vp]),
     "sft_quantize_i16": (ctypes.c_int, [_vp, _i64, ctypes.c_float, _vp, _vp]),
-    "sft_linear_fwd_workspace_size": (ctypes.c_int, [_i32, _i64, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)]),
+    "sft_linear_fwd_workspace_size": (
+        ctypes.c_int, [_i32, _i64, _i64, _i64, _u32, ctypes.POINTER(ctypes.c_size_t)]),
     "sft_linear_fwd": (
         ctypes.c_int,
         [_i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, ctypes.c_size_t,
          _vp]),
     "sft_linear_bwd_workspace_size": (
-        ctypes.c_int, [_i32, _i64, _i64, _i64, _i32, ctypes.POINTER(ctypes.c_size_t)]),
+        ctypes.c_int, [_i32, _i64, _i64, _i64, _i32, _u32, ctypes.POINTER(ctypes.c_size_t)]),
     "sft_linear_bwd": (
         ctypes.c_int,
         [_i32, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, ctypes.c_size_t,
@@ -773,7 +775,10 @@ def quantize_i16(x: torch.Tensor, scale: float) -> torch.Tensor:
 
 
 # ---- the dense head ----
+# Small calls of these are bound by the host, so pointers and streams go as plain
+# integers and the device is set only where it is not the current one.
 _TYPES = {torch.float32: SFT_TYPE_F32, torch.float16: SFT_TYPE_F16, torch.bfloat16: SFT_TYPE_BF16}
+_SIZES = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
 
 
 def type_code(dtype: torch.dtype) -> int:
@@ -782,11 +787,37 @@ def type_code(dtype: torch.dtype) -> int:
     return code
 
 
-def _rows(t: torch.Tensor):
+def _call(name: str, device: torch.device, *args) -> None:
+    """lib().name(*args, stream): on the tensors' device and its current stream."""
+    fn = getattr(_lib or lib(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != SFT_OK:
+        _check(rc, name)
+
+
+def _at(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t: torch.Tensor) -> int:
     """Row stride of a 2-D tensor whose rows are dense (a tensor of one row or column has any)."""
-    rows, cols = t.shape
-    _require(cols == 1 or t.stride(1) == 1, "rows must be dense (stride 1 in the last dimension)")
-    return t.stride(0) if rows > 1 and t.stride(0) >= cols else cols
+    (rows, cols), (ld, step) = t.shape, t.stride()
+    if cols != 1 and step != 1:
+        raise ValueError("rows must be dense (stride 1 in the last dimension)")
+    return ld if rows > 1 and ld >= cols else cols
+
+
+def _copy_flag(*operands: torch.Tensor) -> int:
+    """SFT_LINEAR_COPY if a dense-rows operand is not one that products read in place."""
+    for t in operands:
+        stride = _rows(t) * _SIZES[t.dtype]
+        if (t.data_ptr() | stride) & 15 or stride > 1 << 23:
+            return SFT_LINEAR_COPY
+    return 0
 
 
 def _scratch(nbytes: int, device: torch.device):
@@ -800,66 +831,57 @@ def _scratch(nbytes: int, device: torch.device):
 def linear_fwd(x, w, bias, residual, y, deriv, act: int) -> None:
     """y = residual + act(x w^T + bias) of 2-D tensors with dense rows; deriv (or None) gets act'."""
     (M, K), N = x.shape, w.shape[0]
-    code = type_code(x.dtype)
-    dev = x.device
-    n = ctypes.c_size_t(0)
-    _check(lib().sft_linear_fwd_workspace_size(code, M, K, N, ctypes.byref(n)), "sft_linear_fwd_workspace_size")
-    with torch.cuda.device(dev):
-        keep, ws = _scratch(n.value, dev)
-        _check(lib().sft_linear_fwd(code, _ptr(x), _rows(x), _ptr(w), _rows(w), _ptr(bias), _ptr(residual),
-                                    0 if residual is None else _rows(residual), _ptr(y), _rows(y), _ptr(deriv), M, K,
-                                    N, act, ws, n.value, _stream(dev)), "sft_linear_fwd")
+    code, dev = type_code(x.dtype), x.device
+    nbytes, keep, ws = 0, None, None
+    if M > 64:  # fewer rows need none
+        n = ctypes.c_size_t(0)
+        _check(lib().sft_linear_fwd_workspace_size(code, M, K, N, _copy_flag(x, w), ctypes.byref(n)),
+               "sft_linear_fwd_workspace_size")
+        nbytes = n.value
+        keep, ws = _scratch(nbytes, dev)
+    _call("sft_linear_fwd", dev, code, x.data_ptr(), _rows(x), w.data_ptr(), _rows(w), _at(bias), _at(residual),
+          0 if residual is None else _rows(residual), y.data_ptr(), _rows(y), _at(deriv), M, K, N, act, ws, nbytes)
     del keep
 
 
 def linear_bwd(dy, deriv, x, w, dx, dw, db, act: int) -> None:
     """dx, dw and db (each may be None) of linear_fwd's y from dy and its deriv."""
     (M, K), N = x.shape, w.shape[0]
-    code = type_code(dy.dtype)
-    dev = dy.device
+    code, dev = type_code(dy.dtype), dy.device
     n = ctypes.c_size_t(0)
-    _check(lib().sft_linear_bwd_workspace_size(code, M, K, N, act, ctypes.byref(n)), "sft_linear_bwd_workspace_size")
-    with torch.cuda.device(dev):
-        keep, ws = _scratch(n.value, dev)
-        _check(lib().sft_linear_bwd(code, _ptr(dy), _rows(dy), _ptr(deriv), _ptr(x), _rows(x), _ptr(w), _rows(w),
-                                    _ptr(dx), _ptr(dw), _ptr(db), M, K, N, act, ws, n.value, _stream(dev)),
-               "sft_linear_bwd")
+    _check(lib().sft_linear_bwd_workspace_size(code, M, K, N, act, _copy_flag(dy, x, w), ctypes.byref(n)),
+           "sft_linear_bwd_workspace_size")
+    keep, ws = _scratch(n.value, dev)
+    _call("sft_linear_bwd", dev, code, dy.data_ptr(), _rows(dy), _at(deriv), x.data_ptr(), _rows(x), w.data_ptr(),
+          _rows(w), _at(dx), _at(dw), _at(db), M, K, N, act, ws, n.value)
     del keep
 
 
 def balance_fwd(logits, mask, top_k: int, loss, counts, kept) -> None:
     """loss (float32), counts (int64 [E]) and kept (int64) of the router's 2-D logits; mask bool [T] or None."""
     T, E = logits.shape
-    code = type_code(logits.dtype)
-    dev = logits.device
+    code, dev = type_code(logits.dtype), logits.device
     n = ctypes.c_size_t(0)
     _check(lib().sft_balance_fwd_workspace_size(code, T, E, ctypes.byref(n)), "sft_balance_fwd_workspace_size")
-    with torch.cuda.device(dev):
-        keep, ws = _scratch(n.value, dev)
-        _check(lib().sft_balance_fwd(code, _ptr(logits), _rows(logits), _ptr(mask), T, E, top_k, _ptr(loss),
-                                     _ptr(counts), _ptr(kept), ws, n.value, _stream(dev)), "sft_balance_fwd")
+    keep, ws = _scratch(n.value, dev)
+    _call("sft_balance_fwd", dev, code, logits.data_ptr(), _rows(logits), _at(mask), T, E, top_k, loss.data_ptr(),
+          counts.data_ptr(), kept.data_ptr(), ws, n.value)
     del keep
 
 
 def balance_bwd(logits, mask, top_k: int, counts, kept, grad_loss, grad_logits) -> None:
     """grad_logits (dense) of balance_fwd's loss times grad_loss (float32 on the device)."""
     T, E = logits.shape
-    dev = logits.device
-    with torch.cuda.device(dev):
-        _check(lib().sft_balance_bwd(type_code(logits.dtype), _ptr(logits), _rows(logits), _ptr(mask), T, E, top_k,
-                                     _ptr(counts), _ptr(kept), _ptr(grad_loss), _ptr(grad_logits), _stream(dev)),
-               "sft_balance_bwd")
+    _call("sft_balance_bwd", logits.device, type_code(logits.dtype), logits.data_ptr(), _rows(logits), _at(mask), T, E,
+          top_k, counts.data_ptr(), kept.data_ptr(), grad_loss.data_ptr(), grad_logits.data_ptr())
 
 
 def distill(student, teacher, indices, temperature: float, row_weight, loss, grad_student) -> None:
     """loss (float32 [R]) and grad_student (dense), each may be None, of 2-D logits and a teacher's dense top ones."""
     R, V = student.shape
-    dev = student.device
-    with torch.cuda.device(dev):
-        _check(lib().sft_distill(type_code(student.dtype), _ptr(student), _rows(student), type_code(teacher.dtype),
-                                 _ptr(teacher), _ptr(indices), indices.element_size(), R, V, teacher.shape[1],
-                                 temperature, _ptr(row_weight), _ptr(loss), _ptr(grad_student), _stream(dev)),
-               "sft_distill")
+    _call("sft_distill", student.device, type_code(student.dtype), student.data_ptr(), _rows(student),
+          type_code(teacher.dtype), teacher.data_ptr(), indices.data_ptr(), indices.element_size(), R, V,
+          teacher.shape[1], temperature, _at(row_weight), _at(loss), _at(grad_student))
 
 
 # ---- per-launch kernel timing ----

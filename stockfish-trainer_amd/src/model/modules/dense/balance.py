@@ -21,7 +21,7 @@ from torch import Tensor, autograd
 
 from sft_amd import _native
 
-from . import ops  # noqa: F401  (registers torch.ops.sft.*)
+from .ops import calls
 from .rows import dense_rows
 
 
@@ -31,7 +31,7 @@ class ExpertBalanceFunction(autograd.Function):
     @staticmethod
     def forward(ctx, logits, mask, top_k):
         logits = dense_rows(logits)
-        loss, counts, kept = torch.ops.sft.balance_fwd(logits, mask, top_k)
+        loss, counts, kept = calls().balance_fwd(logits, mask, top_k)
         ctx.save_for_backward(logits, mask, counts, kept)
         ctx.top_k = top_k
         ctx.mark_non_differentiable(counts)
@@ -41,7 +41,7 @@ class ExpertBalanceFunction(autograd.Function):
     @autograd.function.once_differentiable
     def backward(ctx, grad_loss, _):
         logits, mask, counts, kept = ctx.saved_tensors
-        return torch.ops.sft.balance_bwd(logits, mask, ctx.top_k, counts, kept, grad_loss.float()), None, None
+        return calls().balance_bwd(logits, mask, ctx.top_k, counts, kept, grad_loss.float()), None, None
 
 
 def expert_balance(logits: Tensor, top_k: int = 1, mask: Tensor | None = None) -> tuple[Tensor, Tensor]:

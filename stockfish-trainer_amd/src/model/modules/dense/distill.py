@@ -26,7 +26,7 @@ from torch import Tensor, autograd
 
 from sft_amd import _native
 
-from . import ops  # noqa: F401  (registers torch.ops.sft.*)
+from .ops import calls
 from .rows import dense_rows
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
@@ -39,13 +39,13 @@ class DistillFunction(autograd.Function):
     def forward(ctx, student, teacher, indices, temperature):
         ctx.save_for_backward(student, teacher, indices)
         ctx.temperature = temperature
-        return torch.ops.sft.distill_loss(student, teacher, indices, temperature)
+        return calls().distill_loss(student, teacher, indices, temperature)
 
     @staticmethod
     @autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         student, teacher, indices = ctx.saved_tensors
-        return torch.ops.sft.distill_grad(student, teacher, indices, ctx.temperature,
+        return calls().distill_grad(student, teacher, indices, ctx.temperature,
                                           grad_loss.float().contiguous()), None, None, None
 
 
@@ -79,4 +79,4 @@ def distill_loss_and_grad(student_logits: Tensor, teacher_logits: Tensor, teache
         assert row_weight.shape == (student.shape[0],) and row_weight.dtype == torch.float32
         assert row_weight.device == student.device
         row_weight = row_weight.detach().contiguous()
-    return torch.ops.sft.distill_loss_and_grad(student.detach(), teacher, indices, float(temperature), row_weight)
+    return calls().distill_loss_and_grad(student.detach(), teacher, indices, float(temperature), row_weight)

@@ -20,7 +20,7 @@ from torch import Tensor, autograd
 
 from sft_amd import _native
 
-from . import ops  # noqa: F401  (registers torch.ops.sft.*)
+from .ops import calls
 from .rows import dense_rows
 
 ACTIVATIONS = {
@@ -40,7 +40,7 @@ class FusedLinearFunction(autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         x, weight, residual = dense_rows(x), dense_rows(weight), dense_rows(residual)
         bias = None if bias is None else bias.contiguous()
-        y, deriv = torch.ops.sft.linear_fwd(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        y, deriv = calls().linear_fwd(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, deriv)
         ctx.act = act
         return y
@@ -52,7 +52,7 @@ class FusedLinearFunction(autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            dx, dw, db = torch.ops.sft.linear_bwd(dense_rows(grad_y), deriv, x, weight, ctx.act, *need[:3])
+            dx, dw, db = calls().linear_bwd(dense_rows(grad_y), deriv, x, weight, ctx.act, *need[:3])
         return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None,
                 grad_y if need[3] else None, None)
 
@@ -67,11 +67,11 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     N, K = weight.shape
     assert N > 0 and K > 0
     lead = x.shape[:-1]
-    for t in (x, weight, bias, residual):
+    dtype, device = x.dtype, x.device
+    assert x.is_cuda and dtype in (torch.float32, torch.float16, torch.bfloat16)
+    for t in (weight, bias, residual):
         if t is not None:
-            assert t.is_cuda and t.device == x.device
-            assert t.dtype == x.dtype
-    assert x.dtype in (torch.float32, torch.float16, torch.bfloat16)
+            assert t.device == device and t.dtype == dtype
     if bias is not None:
         assert bias.shape == (N,)
     if residual is not None:
@@ -84,6 +84,6 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     else:
         # nothing to record: straight to the library
         x, weight, residual = dense_rows(x), dense_rows(weight), dense_rows(residual)
-        y = torch.empty(x.shape[0], N, dtype=x.dtype, device=x.device)
+        y = torch.empty(x.shape[0], N, dtype=dtype, device=device)
         _native.linear_fwd(x, weight, None if bias is None else bias.contiguous(), residual, y, None, act)
     return y if len(lead) == 1 else y.view(*lead, N)
