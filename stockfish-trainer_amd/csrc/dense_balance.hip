@@ -29,26 +29,31 @@ using dense::group_sum;
 constexpr int kThreads = 1024;   // of the forward: 16 waves, whose sums leave as one partial
 constexpr int kMaxParts = 256;  // its workgroups, one per CU
 
-// A row's logits: lane t of the group holds the chunks t + G j of V elements.
-// Elements past E are -inf.
-template <typename T, int G, int C>
+// A row's logits: lane t of the group holds the chunks t + G j of V elements.  Loads
+// have no branches (whole: E is a multiple of V), so that the next row's are under way
+// beside this one's work; open() turns them into numbers, -inf past E.
+template <typename T, int G, int C, bool WHOLE>
 struct Row {
   static constexpr int V = 16 / (int)sizeof(T);
+  T raw[C][V];
   float x[C][V];
   __device__ __forceinline__ void load(const T *row, int E, int t) {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int e0 = (t + G * j) * V;
-      T v[V];
-      if (e0 + V <= E) {
-        __builtin_memcpy(v, row + e0, 16);
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[j][i] = (float)v[i];
+      if (WHOLE) {
+        __builtin_memcpy(raw[j], row + (e0 < E ? e0 : 0), 16);
       } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[j][i] = e0 + i < E ? (float)row[e0 + i] : -INFINITY;
+        for (int i = 0; i < V; ++i) raw[j][i] = row[e0 + i < E ? e0 + i : 0];
       }
     }
+  }
+  __device__ __forceinline__ void open(int E, int t) {
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[j][i] = (t + G * j) * V + i < E ? (float)raw[j][i] : -INFINITY;
   }
   __device__ __forceinline__ float max() const {
     float m = -INFINITY;
@@ -77,13 +82,13 @@ struct Row {
 };
 
 // part_p [parts][E] sums of p, part_c [parts][E] counts, part_n [parts] kept rows.
-template <typename T, int G, int C>
+template <typename T, int G, int C, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restrict__ logits, int64_t ld,
                                                                const uint8_t *__restrict__ mask, int64_t rows, int E,
                                                                int top_k, float *__restrict__ part_p,
                                                                int32_t *__restrict__ part_c,
                                                                int32_t *__restrict__ part_n) {
-  constexpr int V = Row<T, G, C>::V, kRows = kThreads / G, kWaves = kThreads / kWave;
+  constexpr int V = Row<T, G, C, WHOLE>::V, kRows = kThreads / G, kWaves = kThreads / kWave;
   __shared__ float red_p[kWaves][G * C * V];
   __shared__ int32_t red_c[kWaves][G * C * V];
   __shared__ int32_t red_n[kWaves];
@@ -100,16 +105,21 @@ __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restri
     }
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
-  Row<T, G, C> row, next;
-  auto use = [&](int64_t i) { return i < rows && (!mask || mask[i]); };
-  bool used = use(r);
-  row.load(logits + (used ? r : 0) * ld, used ? E : 0, t);
+  Row<T, G, C, WHOLE> row;
+  uint8_t use = 0, use_next = 0;
+  auto load = [&](int64_t i, uint8_t &u) {  // of a row past the end: the last one's, not used
+    const int64_t at = i < rows ? i : rows - 1;
+    u = mask ? mask[at] : 1;
+    row.load(logits + at * ld, E, t);
+    if (i >= rows) u = 0;
+  };
+  if (rows > 0) load(r, use);
   // the whole wave goes round while any of its rows is left
   for (int64_t left = rows - (int64_t)blockIdx.x * kRows - wave * (kWave / G); left > 0; left -= step) {
-    const bool use_next = use(r + step);
-    next.load(logits + (use_next ? r + step : 0) * ld, use_next ? E : 0, t);
+    row.open(E, t);
+    load(r + step, use_next);
     const float m = row.max();
-    const bool keep = used && m > -INFINITY;  // the same in all lanes of a group
+    const bool keep = use && m > -INFINITY;  // the same in all lanes of a group
     float p[C][V];
     row.softmax(keep ? m : 0.f, p);
 #pragma unroll
@@ -141,8 +151,7 @@ __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restri
         open = open && !hits;
       }
     }
-    row = next;
-    used = use_next;
+    use = use_next;
     r += step;
   }
   // Sums over the row groups of the wave, then over the waves.
@@ -242,13 +251,13 @@ __global__ __launch_bounds__(kJoin) void balance_join_kernel(const float *__rest
   }
 }
 
-template <typename T, int G, int C>
+template <typename T, int G, int C, bool WHOLE>
 __global__ __launch_bounds__(kBlock) void balance_bwd_kernel(const T *__restrict__ logits, int64_t ld,
                                                              const uint8_t *__restrict__ mask, int64_t rows, int E,
                                                              int top_k, const int64_t *__restrict__ counts,
                                                              const int64_t *__restrict__ kept,
                                                              const float *__restrict__ grad, T *__restrict__ out) {
-  constexpr int V = Row<T, G, C>::V, kRows = kBlock / G;
+  constexpr int V = Row<T, G, C, WHOLE>::V, kRows = kBlock / G;
   const int t = lane_id() % G;
   const double n = (double)*kept;
   const float share = n > 0 ? (float)(1.0 / (n * top_k)) : 0.f;
@@ -261,13 +270,22 @@ __global__ __launch_bounds__(kBlock) void balance_bwd_kernel(const T *__restrict
       const int e = (t + G * j) * V + i;
       f[j][i] = e < E ? (float)counts[e] * share : 0.f;
     }
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
-    const int64_t r = r0 + threadIdx.x / G;
-    const bool use = r < rows && (!mask || mask[r]);
-    Row<T, G, C> row;
-    row.load(logits + (use ? r : 0) * ld, use ? E : 0, t);
+  Row<T, G, C, WHOLE> row;
+  uint8_t use = 0;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
+  auto load = [&](int64_t i) {
+    const int64_t at = i < rows ? i : rows - 1;
+    use = mask ? mask[at] : 1;
+    row.load(logits + at * ld, E, t);
+  };
+  load(r);
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += step, r += step) {
+    row.open(E, t);
+    const uint8_t used = use;
+    load(r + step);
     const float m = row.max();
-    const bool keep = use && m > -INFINITY;
+    const bool keep = used && m > -INFINITY;
     float p[C][V];
     row.softmax(keep ? m : 0.f, p);
     float dot = 0.f;
@@ -318,12 +336,12 @@ void row_shape(int E, int V, int *G, int *C) {
   while (*G * *C < chunks) *C *= 2;
 }
 
-template <typename T, int G, int C>
+template <typename T, int G, int C, bool WHOLE>
 void launch(const Call &c, int parts, hipStream_t s) {
   const T *logits = static_cast<const T *>(c.logits);
   if (c.out) {
     const int64_t blocks = ceil_div(c.rows, kBlock / G);
-    hipLaunchKernelGGL((balance_bwd_kernel<T, G, C>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kBlock), 0,
+    hipLaunchKernelGGL((balance_bwd_kernel<T, G, C, WHOLE>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kBlock), 0,
                        s, logits, c.ld, c.mask, c.rows, c.E, c.top_k, c.counts, c.kept, c.grad,
                        static_cast<T *>(c.out));
     return;
@@ -331,7 +349,7 @@ void launch(const Call &c, int parts, hipStream_t s) {
   float *part_p = static_cast<float *>(c.ws);
   int32_t *part_c = reinterpret_cast<int32_t *>(part_p + (int64_t)parts * c.E);
   int32_t *part_n = part_c + (int64_t)parts * c.E;
-  hipLaunchKernelGGL((balance_fwd_kernel<T, G, C>), dim3(parts), dim3(kThreads), 0, s, logits, c.ld, c.mask, c.rows,
+  hipLaunchKernelGGL((balance_fwd_kernel<T, G, C, WHOLE>), dim3(parts), dim3(kThreads), 0, s, logits, c.ld, c.mask, c.rows,
                      c.E, c.top_k, part_p, part_c, part_n);
   hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(kJoin), 0, s, part_p, part_c, part_n, parts, c.E, c.top_k,
                      c.loss, c.counts, c.kept);
@@ -350,7 +368,7 @@ void launch_type(const Call &c, hipStream_t s) {
   int G, C;
   row_shape(c.E, 16 / (int)sizeof(T), &G, &C);
 #define SFT_BALANCE(g, k) \
-  if (G == g && C == k) return launch<T, g, k>(c, parts, s)
+  if (G == g && C == k) return c.E % (16 / (int)sizeof(T)) ? launch<T, g, k, false>(c, parts, s) : launch<T, g, k, true>(c, parts, s)
   SFT_BALANCE(1, 1);
   SFT_BALANCE(2, 1);
   SFT_BALANCE(4, 1);

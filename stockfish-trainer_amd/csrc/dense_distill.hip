@@ -12,7 +12,9 @@
 // comes, with a running maximum and sum per thread, and stays in the registers of the
 // waves that hold it, as loaded, until the gradient; rows longer than a workgroup's
 // registers are read again, from L2 or the memory-side cache.  Rows start anywhere, so
-// chunks are cut where the gradient's (without one: the logits') 16-byte lines are.
+// they are cut at the logits' 16-byte lines: whole chunks, and the few elements before
+// and after them one a thread.  All loads of a row
+// are made without branches, so that they are under way together.
 #include "dense.h"
 #include "dense_reduce.h"
 
@@ -134,20 +136,6 @@ struct Teacher {
   }
 };
 
-// The chunk of V elements of a row of n whose first is number `at` (it may hang over
-// either end); -inf outside the row.
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T *row, int at, int n, u32x4 &v) {
-  constexpr int V = 16 / (int)sizeof(T);
-  if (at >= 0 && at + V <= n) {
-    __builtin_memcpy(&v, row + at, 16);
-  } else {
-    T e[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = at + i >= 0 && at + i < n ? row[at + i] : (T)(-INFINITY);
-    __builtin_memcpy(&v, e, 16);
-  }
-}
 template <typename T>
 __device__ __forceinline__ void unpack(const u32x4 &v, float (&x)[16 / sizeof(T)]) {
   T e[16 / sizeof(T)];
@@ -156,18 +144,13 @@ __device__ __forceinline__ void unpack(const u32x4 &v, float (&x)[16 / sizeof(T)
   for (int i = 0; i < 16 / (int)sizeof(T); ++i) x[i] = (float)e[i];
 }
 template <typename T>
-__device__ __forceinline__ void store_chunk(T *row, int at, int n, const float (&x)[16 / sizeof(T)]) {
-  constexpr int V = 16 / (int)sizeof(T);
-  T e[V];
+__device__ __forceinline__ u32x4 pack(const float (&x)[16 / sizeof(T)]) {
+  T e[16 / sizeof(T)];
 #pragma unroll
-  for (int i = 0; i < V; ++i) e[i] = (T)x[i];
-  if (at >= 0 && at + V <= n) {
-    __builtin_memcpy(row + at, e, 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (at + i >= 0 && at + i < n) row[at + i] = e[i];
-  }
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i) e[i] = (T)x[i];
+  u32x4 v;
+  __builtin_memcpy(&v, e, 16);
+  return v;
 }
 
 // TPR threads per row (one wave, or the whole workgroup of TPR), C chunks a thread.
@@ -184,34 +167,55 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
   if (row >= d.rows) return;  // whole waves, and never part of a row's
   const T *s = static_cast<const T *>(d.s) + row * d.lds;
   T *ds = static_cast<T *>(d.ds) + row * (int64_t)d.V;
-  // chunk c holds the elements from c V - shift on
-  const int shift = (int)((uintptr_t)(d.ds ? ds : s) / sizeof(T) % V);
-  const int chunks = (d.V + shift + V - 1) / V;
+  // `head` elements, whole chunks, and the rest; thread i < edge has one of the others
+  const int shift = (int)((uintptr_t)s / sizeof(T) % V);
+  int head = shift ? V - shift : 0;
+  head = head < d.V ? head : d.V;
+  const int body = (d.V - head) / V, edge = d.V - body * V;
+  const int mine = tid < head ? tid : d.V - edge + tid;
+  const T *sb = s + head;
+  T *dsb = ds + head;
   const float c2 = 1.44269504088896341f / d.tau;  // exp(x / tau) = 2^(x c2)
 
+  T nothing[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) nothing[i] = (T)(-INFINITY);
+  u32x4 none;
+  __builtin_memcpy(&none, nothing, 16);
   u32x4 raw[C ? C : 1];
   if (C) {
 #pragma unroll
-    for (int j = 0; j < C; ++j) load_chunk<T>(s, (tid + TPR * j) * V - shift, d.V, raw[j]);
+    for (int j = 0; j < C; ++j) {
+      const int c = tid + TPR * j;
+      if (body > 0) __builtin_memcpy(&raw[j], sb + (int64_t)(c < body ? c : body - 1) * V, 16);
+    }
   }
+  float x_edge = (float)s[tid < edge ? mine : 0];
+  if (tid >= edge) x_edge = -INFINITY;
   Teacher te;
   if (wave == 0) te.load(d, row, s);
   Running run;
   if (C) {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
+      if (tid + TPR * j >= body) raw[j] = none;
       float x[V];
       unpack<T>(raw[j], x);
       run.add(x, c2);
     }
   } else {
-    for (int c = tid; c < chunks; c += TPR) {
+#pragma unroll 4
+    for (int c = tid; c < body; c += TPR) {
       u32x4 v;
       float x[V];
-      load_chunk<T>(s, c * V - shift, d.V, v);
+      __builtin_memcpy(&v, sb + (int64_t)c * V, 16);
       unpack<T>(v, x);
       run.add(x, c2);
     }
+  }
+  {
+    const float x[1] = {x_edge};
+    run.add(x, c2);
   }
   run.join(c2);
   if (kWaves > 1) {
@@ -238,24 +242,28 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
   if (!d.ds) return;
 
   const float g = d.tau * (d.weight ? d.weight[row] : 1.f), gp = g / sum;
+  auto grad = [&](float x) { return live ? gp * __builtin_amdgcn_exp2f((x - m) * c2) : 0.f; };
   auto put = [&](int c, const u32x4 &v) {
     float x[V];
     unpack<T>(v, x);
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = live ? gp * __builtin_amdgcn_exp2f((x[i] - m) * c2) : 0.f;
-    store_chunk<T>(ds, c * V - shift, d.V, x);
+    for (int i = 0; i < V; ++i) x[i] = grad(x[i]);
+    const u32x4 e = pack<T>(x);
+    __builtin_memcpy(dsb + (int64_t)c * V, &e, 16);
   };
   if (C) {
 #pragma unroll
     for (int j = 0; j < C; ++j)
-      if (tid + TPR * j < chunks) put(tid + TPR * j, raw[j]);
+      if (tid + TPR * j < body) put(tid + TPR * j, raw[j]);
   } else {
-    for (int c = tid; c < chunks; c += TPR) {
+#pragma unroll 4
+    for (int c = tid; c < body; c += TPR) {
       u32x4 v;
-      load_chunk<T>(s, c * V - shift, d.V, v);
+      __builtin_memcpy(&v, sb + (int64_t)c * V, 16);
       put(c, v);
     }
   }
+  if (tid < edge) ds[mine] = (T)grad(x_edge);
   if (!live) return;  // the same for the whole row
   // The teacher's classes once more, after the stores above have been made.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -272,9 +280,7 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
 template <typename T>
 void launch(const Distill &d, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
-  // rows may start inside a chunk
-  const bool whole = ((uintptr_t)(d.ds ? d.ds : d.s) % 16 | (uintptr_t)((d.ds ? d.V : d.lds) % V)) == 0;
-  const int64_t chunks = ceil_div(d.V, V) + !whole;
+  const int64_t chunks = d.V / V;
 #define SFT_DISTILL(most, TPR, C)                                                                                  \
   if (chunks <= most) {                                                                                            \
     hipLaunchKernelGGL((distill_kernel<T, TPR, C>),                                                                \
@@ -282,7 +288,7 @@ void launch(const Distill &d, hipStream_t s) {
                        dim3(TPR == kWave ? kBlock : TPR), 0, s, d);                                                \
     return;                                                                                                        \
   }
-  SFT_DISTILL(64, 64, 1)
+  SFT_DISTILL(64, 64, 1)  // an edge of up to 14 elements fits any wave
   SFT_DISTILL(128, 64, 2)
   SFT_DISTILL(256, 64, 4)
   SFT_DISTILL(512, 64, 8)

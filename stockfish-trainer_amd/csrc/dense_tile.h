@@ -60,10 +60,15 @@ __device__ __forceinline__ void activate(float (&z)[V], float (&d)[V], int act) 
       }
       break;
     case SFT_ACT_GELU:
+      // erfc by the rational approximation 7.1.26 of Abramowitz and Stegun, within
+      // 1.5e-7; its exponential is the derivative's too.
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float cdf = 0.5f * (1.f + erff(z[i] * 0.70710678118654752f));
-        d[i] = cdf + z[i] * (0.39894228040143268f * expf(-0.5f * z[i] * z[i]));
+        const float a = fabsf(z[i]) * 0.70710678118654752f, e = expf(-a * a), t = 1.f / (1.f + 0.3275911f * a);
+        const float tail =
+            0.5f * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * e;
+        const float cdf = z[i] < 0.f ? tail : 1.f - tail;
+        d[i] = cdf + z[i] * (0.39894228040143268f * e);
         z[i] *= cdf;
       }
       break;
@@ -542,38 +547,52 @@ __global__ __launch_bounds__(kBlock) void gemm_join_kernel(const Gemm g) {
 constexpr int kRowWaves = 8;
 template <typename T, int FM>
 __global__ __launch_bounds__(kRowWaves *kWave) void gemm_rows_kernel(const Gemm g) {
-  constexpr int kEpc = 16 / (int)sizeof(T), kPiece = 16 * kEpc;
+  constexpr int kEpc = 16 / (int)sizeof(T);
   __shared__ f32x4 red[kRowWaves][FM][kWave];
   const int lane = lane_id(), i = lane % 16, c = lane / 16;
   const int wave = uniform(threadIdx.x / kWave);
   const int n0 = blockIdx.x * 16;
-  const bool nin = n0 + i < g.N;
-  const T *w = static_cast<const T *>(g.b) + (int64_t)(nin ? n0 + i : 0) * g.ldb;
+  // rows and columns past the last: its own again, not stored
+  const T *w = static_cast<const T *>(g.b) + (int64_t)(n0 + i < g.N ? n0 + i : g.N - 1) * g.ldb;
   const T *x[FM];
-  bool in[FM];
 #pragma unroll
-  for (int f = 0; f < FM; ++f) {
-    in[f] = f * 16 + i < g.M;
-    x[f] = static_cast<const T *>(g.a) + (int64_t)(in[f] ? f * 16 + i : 0) * g.lda;
-  }
-  f32x4 acc[FM];
+  for (int f = 0; f < FM; ++f) x[f] = static_cast<const T *>(g.a) + (int64_t)(f * 16 + i < g.M ? f * 16 + i : g.M - 1) * g.lda;
+  f32x4 acc[FM] = {};
+  auto products = [&](const Frag<T> &fw, const Frag<T>(&fx)[FM]) {
 #pragma unroll
-  for (int f = 0; f < FM; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k0 = wave * kPiece; k0 < g.K; k0 += kRowWaves * kPiece) {
-    Frag<T> fw[4], fx[FM][4];
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+      for (int t = 0; t < Mma<T>::kSteps; ++t) acc[f] = Mma<T>::step(fw, fx[f], acc[f], t);
+  };
+  // Whole chunks: loads without branches, so that a piece's are under way together;
+  // what lies past them is read as the last one and not used.
+  const int whole = g.K / kEpc;
+  for (int q0 = wave * 16; q0 < whole; q0 += kRowWaves * 16) {
+    Frag<T> fw[4], fx[4][FM];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int k = k0 + (u * 4 + c) * kEpc;
-      fw[u].v = load_chunk(w + k, nin ? g.K - k : 0);
+      const int q = q0 + u * 4 + c, at = (q < whole ? q : whole - 1) * kEpc;
+      __builtin_memcpy(&fw[u].v, w + at, 16);
 #pragma unroll
-      for (int f = 0; f < FM; ++f) fx[f][u].v = load_chunk(x[f] + k, in[f] ? g.K - k : 0);
+      for (int f = 0; f < FM; ++f) __builtin_memcpy(&fx[u][f].v, x[f] + at, 16);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u) {
+      if (q0 + u * 4 + c >= whole) {
+        fw[u].v = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int f = 0; f < FM; ++f)
+        for (int f = 0; f < FM; ++f) fx[u][f].v = u32x4{0u, 0u, 0u, 0u};
+      }
+      products(fw[u], fx[u]);
+    }
+  }
+  if (wave == kRowWaves - 1 && g.K % kEpc) {  // the last elements
+    Frag<T> fw, fx[FM];
+    const int at = whole * kEpc, cnt = c == 0 ? g.K - at : 0;
+    fw.v = load_chunk(w + at, cnt);
 #pragma unroll
-        for (int t = 0; t < Mma<T>::kSteps; ++t) acc[f] = Mma<T>::step(fw[u], fx[f][u], acc[f], t);
+    for (int f = 0; f < FM; ++f) fx[f].v = load_chunk(x[f] + at, cnt);
+    products(fw, fx);
   }
 #pragma unroll
   for (int f = 0; f < FM; ++f) red[wave][f][lane] = acc[f];
