@@ -13,7 +13,7 @@ namespace {
 constexpr int kStage = 64;         // bytes of k per pipeline stage
 constexpr int64_t kRowsMost = 64;  // rows the row kernel takes
 constexpr int64_t kCus = 256;
-constexpr int64_t kStrideMost = (int64_t)1 << 23;  // bytes: a tile's rows stay within 31-bit offsets
+constexpr int64_t kStrideMost = (int64_t)1 << 23;  // bytes: a tile's rows span less than 32 bits count
 
 size_t a256(size_t n) { return (n + 255) & ~(size_t)255; }
 int64_t type_size(int dtype) { return dtype == SFT_TYPE_F32 ? 4 : 2; }
@@ -36,8 +36,8 @@ struct TileCost {
   int rows, cols, slots;              // slots: workgroups the card holds at once
   double stage[2], alone[2], round;   // us a stage of 16-bit types and of binary32, with many and one per CU
 };
-constexpr TileCost kTiles[3] = {{64, 128, 768, {0.17, 0.50}, {0.26, 0.57}, 4.0},
-                                {128, 128, 768, {0.29, 0.95}, {0.42, 1.00}, 5.0},
+constexpr TileCost kTiles[3] = {{64, 128, 768, {0.17, 0.42}, {0.26, 0.58}, 4.0},
+                                {128, 128, 768, {0.29, 0.70}, {0.42, 0.60}, 5.0},
                                 {256, 256, 256, {0.84, 0.0}, {0.84, 0.0}, 8.0}};
 Cut cut_of(int dtype, int64_t M, int64_t N, int64_t K) {
   const int64_t es = type_size(dtype), stages = ceil_div(K * es, kStage);
@@ -249,8 +249,8 @@ int linear_bwd(int dtype, const void *dy, int64_t lddy, const void *deriv, const
     rc = SFT_DENSE_CALL(dtype, launch_act_bwd, p, db, s);
   }
   Matrix in{x, ldx, M, K}, weight{w, ldw, N, K};
-  if (!rc && (dx || dw)) rc = align(dtype, &dz, dx ? &weight : nullptr, ws, s);
-  if (!rc && dw) rc = align(dtype, &in, nullptr, ws, s);
+  if (!rc && (dx || dw)) rc = align(dtype, &dz, nullptr, ws, s);
+  if (!rc) rc = align(dtype, dx ? &weight : nullptr, dw ? &in : nullptr, ws, s);
   if (!rc && dx)
     rc = run_gemm(dtype, kInputGrad, dz, weight, M, K, N,
                   Epilogue{nullptr, nullptr, dx, nullptr, 0, K, SFT_ACT_NONE, false}, ws, s);

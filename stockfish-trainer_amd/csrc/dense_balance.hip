@@ -81,13 +81,68 @@ struct Row {
   }
 };
 
+// One workgroup: counts, the number of kept rows and the loss from the partials.
+// Threads (slice, expert): a slice adds every kSlices-th partial, the slices are
+// added in order.
+__device__ __forceinline__ void join_parts(const float *part_p, const int32_t *part_c, const int32_t *part_n, int parts,
+                                           int E, int top_k, float *loss, int64_t *counts, int64_t *kept) {
+  __shared__ double red_p[kThreads];
+  __shared__ int64_t red_c[kThreads];
+  __shared__ double sums[kThreads / kWave];
+  const int tid = threadIdx.x;
+  int width = 1;
+  while (width < E) width <<= 1;  // <= kThreads
+  const int slices = kThreads / width, e = tid % width, slice = tid / width;
+  // kept rows: wave 0 adds the parts
+  int64_t n = 0;
+  for (int i = tid; i < parts; i += kThreads) n += part_n[i];
+  red_c[tid] = n;
+  __syncthreads();
+  for (int d = kThreads / 2; d > 0; d >>= 1) {
+    if (tid < d) red_c[tid] += red_c[tid + d];
+    __syncthreads();
+  }
+  n = red_c[0];
+  __syncthreads();
+  double p = 0.0;
+  int64_t c = 0;
+  if (e < E) {
+#pragma unroll 8
+    for (int i = slice; i < parts; i += slices) {
+      p += (double)part_p[(int64_t)i * E + e];
+      c += part_c[(int64_t)i * E + e];
+    }
+  }
+  red_p[tid] = p;
+  red_c[tid] = c;
+  __syncthreads();
+  double term = 0.0;
+  if (slice == 0 && e < E) {
+    for (int i = 1; i < slices; ++i) {
+      p += red_p[i * width + e];
+      c += red_c[i * width + e];
+    }
+    counts[e] = c;
+    term = (double)c * p;
+  }
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) term += __shfl_xor(term, m);
+  if (tid % kWave == 0) sums[tid / kWave] = term;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < kThreads / kWave; ++i) term += sums[i];
+    *kept = n;
+    *loss = n ? (float)(term * E / ((double)n * (double)n * top_k)) : 0.f;
+  }
+}
+
 // part_p [parts][E] sums of p, part_c [parts][E] counts, part_n [parts] kept rows.
 template <typename T, int G, int C, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restrict__ logits, int64_t ld,
                                                                const uint8_t *__restrict__ mask, int64_t rows, int E,
-                                                               int top_k, float *__restrict__ part_p,
-                                                               int32_t *__restrict__ part_c,
-                                                               int32_t *__restrict__ part_n) {
+                                                               int top_k, float *part_p, int32_t *part_c, int32_t *part_n,
+                                                               float *loss,
+                                                               int64_t *counts, int64_t *kept_rows) {
   constexpr int V = Row<T, G, C, WHOLE>::V, kRows = kThreads / G, kWaves = kThreads / kWave;
   __shared__ float red_p[kWaves][G * C * V];
   __shared__ int32_t red_c[kWaves][G * C * V];
@@ -189,66 +244,19 @@ __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restri
     for (int w = 0; w < kWaves; ++w) n += red_n[w];
     part_n[blockIdx.x] = n;
   }
+  if (gridDim.x > 1) return;
+  __threadfence_block();
+  __syncthreads();
+  join_parts(part_p, part_c, part_n, 1, E, top_k, loss, counts, kept_rows);  // the only part: no launch for it
 }
 
-// One workgroup: counts, the number of kept rows and the loss from the partials.
-// Threads (slice, expert): a slice adds every kSlices-th partial, the slices are
-// added in order.
-constexpr int kJoin = 1024;
-__global__ __launch_bounds__(kJoin) void balance_join_kernel(const float *__restrict__ part_p,
-                                                             const int32_t *__restrict__ part_c,
-                                                             const int32_t *__restrict__ part_n, int parts, int E,
-                                                             int top_k, float *__restrict__ loss,
-                                                             int64_t *__restrict__ counts,
-                                                             int64_t *__restrict__ kept) {
-  __shared__ double red_p[kJoin];
-  __shared__ int64_t red_c[kJoin];
-  __shared__ double sums[kJoin / kWave];
-  const int tid = threadIdx.x;
-  int width = 1;
-  while (width < E) width <<= 1;  // <= kJoin
-  const int slices = kJoin / width, e = tid % width, slice = tid / width;
-  // kept rows: wave 0 adds the parts
-  int64_t n = 0;
-  for (int i = tid; i < parts; i += kJoin) n += part_n[i];
-  red_c[tid] = n;
-  __syncthreads();
-  for (int d = kJoin / 2; d > 0; d >>= 1) {
-    if (tid < d) red_c[tid] += red_c[tid + d];
-    __syncthreads();
-  }
-  n = red_c[0];
-  __syncthreads();
-  double p = 0.0;
-  int64_t c = 0;
-  if (e < E) {
-#pragma unroll 8
-    for (int i = slice; i < parts; i += slices) {
-      p += (double)part_p[(int64_t)i * E + e];
-      c += part_c[(int64_t)i * E + e];
-    }
-  }
-  red_p[tid] = p;
-  red_c[tid] = c;
-  __syncthreads();
-  double term = 0.0;
-  if (slice == 0 && e < E) {
-    for (int i = 1; i < slices; ++i) {
-      p += red_p[i * width + e];
-      c += red_c[i * width + e];
-    }
-    counts[e] = c;
-    term = (double)c * p;
-  }
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) term += __shfl_xor(term, m);
-  if (tid % kWave == 0) sums[tid / kWave] = term;
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < kJoin / kWave; ++i) term += sums[i];
-    *kept = n;
-    *loss = n ? (float)(term * E / ((double)n * (double)n * top_k)) : 0.f;
-  }
+__global__ __launch_bounds__(kThreads) void balance_join_kernel(const float *__restrict__ part_p,
+                                                                const int32_t *__restrict__ part_c,
+                                                                const int32_t *__restrict__ part_n, int parts, int E,
+                                                                int top_k, float *__restrict__ loss,
+                                                                int64_t *__restrict__ counts,
+                                                                int64_t *__restrict__ kept) {
+  join_parts(part_p, part_c, part_n, parts, E, top_k, loss, counts, kept);
 }
 
 template <typename T, int G, int C, bool WHOLE>
@@ -350,8 +358,9 @@ void launch(const Call &c, int parts, hipStream_t s) {
   int32_t *part_c = reinterpret_cast<int32_t *>(part_p + (int64_t)parts * c.E);
   int32_t *part_n = part_c + (int64_t)parts * c.E;
   hipLaunchKernelGGL((balance_fwd_kernel<T, G, C, WHOLE>), dim3(parts), dim3(kThreads), 0, s, logits, c.ld, c.mask, c.rows,
-                     c.E, c.top_k, part_p, part_c, part_n);
-  hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(kJoin), 0, s, part_p, part_c, part_n, parts, c.E, c.top_k,
+                     c.E, c.top_k, part_p, part_c, part_n, c.loss, c.counts, c.kept);
+  if (parts > 1)
+    hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(kThreads), 0, s, part_p, part_c, part_n, parts, c.E, c.top_k,
                      c.loss, c.counts, c.kept);
 }
 

@@ -176,54 +176,71 @@ struct TileMap {
 };
 
 // Copies a stage's chunks straight to LDS with bounds-checked buffer loads (out of
-// range reads give zeros).  Rows are 16-byte aligned and hold whole chunks.
+// range reads give zeros).  Rows are 16-byte aligned and hold whole chunks.  What a
+// stage adds to a wave's scalar work delays its products, so ranges are 32-bit (a
+// tile's rows span less) and the end of k is cut once, by clip().
 template <typename T, int BMN, bool KMAJ, int THREADS>
 struct DirectLoader {
   typedef TileMap<T, BMN, KMAJ> Map;
   static constexpr int kLoads = Map::kBytes / 16 / THREADS;
   static_assert(Map::kBytes % (16 * THREADS) == 0, "whole copies");
-  static constexpr uint32_t kOut = 0x80000000u;  // beyond any range below
+  static constexpr uint32_t kOut = 0xffffff00u;  // beyond any range below
   const char *base;
-  int64_t left;  // bytes from base to the end of the operand
   int64_t step;
+  uint32_t range;  // k-major: bytes from base to the end of the tile's rows
+  uint32_t pitch, width;  // row-k: bytes of a row's stride, and of its part in the tile
   uint32_t off[kLoads];
+  int kleft;   // k of the operand from the next stage's first
   int kchunk;  // k-major: first k of this thread's chunk within a stage
-  // mn0: first row of the tile; k0: first k; K: end of the k range.
+  // mn0: first row of the tile; k0: first k; K: end of the operand's k.
   __device__ __forceinline__ void init(const void *p, int64_t ld, int mn0, int MN, int k0, int K) {
     const int tid = threadIdx.x;
+    pitch = (uint32_t)(ld * Map::kEs);
+    kleft = K - k0;
     if (KMAJ) {
+      const int rows = MN - mn0 < BMN ? MN - mn0 : BMN;
       base = static_cast<const char *>(p) + ((int64_t)mn0 * ld + k0) * Map::kEs;
-      left = ((int64_t)(MN - 1 - mn0) * ld + K - k0) * Map::kEs;
+      range = rows > 0 && K > k0 ? (uint32_t)(rows - 1) * pitch + (uint32_t)(K - k0) * Map::kEs : 0u;
       step = kStageBytes;
     } else {
       base = static_cast<const char *>(p) + ((int64_t)k0 * ld + mn0) * Map::kEs;
-      left = ((int64_t)(K - 1 - k0) * ld + MN - mn0) * Map::kEs;
+      width = MN > mn0 ? (uint32_t)(MN - mn0) * Map::kEs : 0u;
       step = (int64_t)Map::kStageK * ld * Map::kEs;
     }
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int q = j * THREADS + tid;
       const int row = q / Map::kRowChunks, c = Map::chunk_at(row, q % Map::kRowChunks);
-      off[j] = (uint32_t)row * (uint32_t)(ld * Map::kEs) + (uint32_t)c * 16u;
+      off[j] = (uint32_t)row * pitch + (uint32_t)c * 16u;
       if (!KMAJ && mn0 + c * Map::kEpc >= MN) off[j] = kOut;
       if (KMAJ) kchunk = c * Map::kEpc;  // the same for every j: THREADS / 4 rows apart
     }
   }
-  // kleft: k from the stage's first to the end of the range.
-  __device__ __forceinline__ void load(SFT_LDS char *lds, int kleft) {
+  // Before a stage with fewer than kStageK k left: the chunks past them.
+  __device__ __forceinline__ void clip() {
+    if (!KMAJ || kleft >= Map::kStageK) return;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) off[j] = kchunk < kleft ? off[j] : kOut;
+  }
+  // lds: the wave's part of the stage.
+  __device__ __forceinline__ void load(SFT_LDS char *lds) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass has no such builtins
-    const uint32_t n = left <= 0 ? 0u : (uint32_t)(left < 0x7ffffff0ll ? left : 0x7ffffff0ll);
+    uint32_t n;
+    if (KMAJ) {
+      n = range;
+      range = (uint32_t)uniform((int)(range > kStageBytes ? range - kStageBytes : 0u));
+    } else {  // the last row's part ends the range
+      const int rows = kleft < Map::kStageK ? kleft : Map::kStageK;
+      n = rows > 0 ? (uint32_t)(rows - 1) * pitch + width : 0u;
+    }
     const __amdgpu_buffer_rsrc_t r =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)n, 0x00020000);
-    const int wave = uniform(threadIdx.x / kWave);
-    const bool in = !KMAJ || kchunk < kleft;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (SFT_LDS void *)(lds + (j * THREADS + wave * kWave) * 16), 16,
-                                               in ? off[j] : kOut, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (SFT_LDS void *)(lds + j * THREADS * 16), 16, off[j], 0, 0, 0);
 #endif
     base += step;
-    left -= step;
+    kleft -= Map::kStageK;
   }
 };
 
@@ -295,6 +312,46 @@ __device__ __forceinline__ void mma_all(const Frag<T> (&fa)[FM], const Frag<T> (
     for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::step(fb[j], fa[i], acc[i][j], s);
+}
+
+// binary32 products on the bfloat16 matrix instructions, whose rate is 16 times that of
+// the binary32 ones: a number is the exact sum of three bfloat16 (8 bits of its 24
+// each, cut off, not rounded), and of the nine partial products the six that reach
+// 2^-24 of the whole are added, in binary32.  What is left out and the sums' own
+// rounding are of the size of a binary32 product's rounding; a row with an infinity
+// becomes NaN (inf - inf) where a binary32 product would keep the infinity.
+// One fragment of each part: 8 k of a lane, 4 from each of two stages.
+struct Split {
+  u32x4 part[3];
+  // The 4 numbers of stage `half` of the pair.
+  __device__ __forceinline__ void take(const u32x4 &raw, int half) {
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      uint32_t a = raw[2 * p], b = raw[2 * p + 1];
+#pragma unroll
+      for (int t = 0; t < 3; ++t) {
+        part[t][2 * half + p] = __builtin_amdgcn_perm(b, a, 0x07060302);  // the upper halves of both
+        if (t == 2) break;
+        const float fa = __builtin_bit_cast(float, a) - __builtin_bit_cast(float, a & 0xffff0000u);
+        const float fb = __builtin_bit_cast(float, b) - __builtin_bit_cast(float, b & 0xffff0000u);
+        a = __builtin_bit_cast(uint32_t, fa);
+        b = __builtin_bit_cast(uint32_t, fb);
+      }
+    }
+#endif
+  }
+};
+// acc[j] += a times b[j], the smallest partial products first.
+template <int FN>
+__device__ __forceinline__ void mma_split(const Split &a, const Split (&b)[FN], f32x4 (&acc)[FN]) {
+  constexpr int kA[6] = {0, 2, 1, 0, 1, 0}, kB[6] = {2, 0, 1, 1, 0, 0};
+#pragma unroll
+  for (int t = 0; t < 6; ++t)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[j].part[kB[t]]),
+                                                       __builtin_bit_cast(bf16x8, a.part[kA[t]]), acc[j], 0, 0, 0);
 }
 
 // Reads the fragments of F consecutive 16-row groups of an LDS tile, from row mn0.
@@ -421,12 +478,13 @@ struct TileWork {
   }
 };
 
-// Aligned operands.  Three things overlap: the copies of stages s + 2 .. s + RING
-// from memory to a ring in LDS, the reads of stage s + 1's fragments into registers,
-// and the products of stage s.  The copies carry their own bounds checks, so those
-// past the end are made too (they give zeros) and every stage waits for the same
-// number of outstanding ones.
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int RING>
+// Three things overlap: the copies of later stages from memory to a ring in LDS, the
+// reads of stage s + 1's fragments into registers, and the products of stage s.  The
+// waves meet once in MEET stages: then the next MEET stages are in LDS, the slots of
+// the past ones are free, and as many copies are made.  The copies carry their own
+// bounds checks, so those past the end are made too (they give zeros) and every
+// meeting waits for the same number of outstanding ones.
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int RING, int MEET>
 __global__ __launch_bounds__(WM *WN *kWave, BM / WM * BN / WN > 128 * 64 ? 1 : 2) void gemm_ring_kernel(const Gemm g) {
   typedef TileWork<T, BM, BN, WM, WN> Work;
   constexpr int FM = Work::FM, FN = Work::FN, kStage = Work::kStage;
@@ -445,75 +503,112 @@ __global__ __launch_bounds__(WM *WN *kWave, BM / WM * BN / WN > 128 * 64 ? 1 : 2
   ra.init(w.wm);
   rb.init(w.wn);
   f32x4 acc[FM][FN] = {};
-  int kleft = w.kend - w.k0;
-  const int steps = (kleft + Work::kStageK - 1) / Work::kStageK;
+  const int steps = (w.kend - w.k0 + Work::kStageK - 1) / Work::kStageK;
   SFT_LDS char *ring = (SFT_LDS char *)lds;
-  // The two slots of one call differ; without the restricts the compiler would wait
-  // for the copies before it reads.
-  auto copy = [&](SFT_LDS char *__restrict__ to) {
-    la.load(to, kleft);
-    lb.load(to + BM * kStageBytes, kleft);
-    kleft -= Work::kStageK;
+  SFT_LDS char *ring_to = ring + uniform(threadIdx.x / kWave) * (kWave * 16);  // the wave's part of a copy
+  int at = 0;  // slot of the next copy
+  auto clip = [&]() {
+    la.clip();
+    lb.clip();
   };
-  auto copy_read = [&](SFT_LDS char *__restrict__ to, const SFT_LDS char *__restrict__ from, Frag<T>(&fa)[FM],
-                       Frag<T>(&fb)[FN]) {
-    la.load(to, kleft);
-    lb.load(to + BM * kStageBytes, kleft);
-    kleft -= Work::kStageK;
+  auto copy = [&](SFT_LDS char *__restrict__ to) {
+    la.load(to);
+    lb.load(to + BM * kStageBytes);
+  };
+  auto read = [&](const SFT_LDS char *__restrict__ from, Frag<T>(&fa)[FM], Frag<T>(&fb)[FN]) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) fa[i] = ra.read(from, i);
 #pragma unroll
     for (int j = 0; j < FN; ++j) fb[j] = rb.read(from + BM * kStageBytes, j);
   };
-  // Own copies up to the last RING - 2 stages' are in LDS and own fragment reads are
-  // done; then the same holds for every wave.
-  auto meet = [&]() {
-    constexpr int kLeft = (RING - 2) * kCopies;
+  // The slots differ; without the restricts the compiler would wait for the copies
+  // before it reads.
+  auto copy_read = [&](SFT_LDS char *__restrict__ to, const SFT_LDS char *__restrict__ from, Frag<T>(&fa)[FM],
+                       Frag<T>(&fb)[FN]) {
+    la.load(to);
+    lb.load(to + BM * kStageBytes);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[i] = ra.read(from, i);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fb[j] = rb.read(from + BM * kStageBytes, j);
+  };
+  // All own copies but those of the last `left` stages are in LDS and own fragment
+  // reads are done; then the same holds for every wave.
+  auto meet = [&](auto left) {
+    constexpr int n = decltype(left)::value * kCopies;
+    static_assert(n < 64, "a 6-bit count");
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((kLeft & 15) | (kLeft >> 4 << 14) | 0x70);  // vmcnt(kLeft) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4 << 14) | 0x70);  // vmcnt(n) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  // The order of one stage: products between the copies and the fragment reads.
+  // The order of one stage: a product or two after each fragment read, then after each
+  // copy, and the rest of the products, in whose time the last reads arrive.
   auto interleave = []() {
     constexpr int kReads = FM * (AK ? 1 : sizeof(T) == 2 ? 2 : 4) + FN * (BK ? 1 : sizeof(T) == 2 ? 2 : 4);
-    constexpr int kProducts = FM * FN * Mma<T>::kSteps, kGroups = kReads + kCopies;
-    constexpr int kPer = kProducts / kGroups > 0 ? kProducts / kGroups : 1;
+    constexpr int kProducts = FM * FN * Mma<T>::kSteps;
+    constexpr int kPer = 2 * kReads > kProducts ? 2 : 1;  // reads a product
+#pragma unroll
+    for (int i = 0; i < kReads / kPer; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);  // LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // matrix instruction
+    }
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // memory read
-      __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);  // matrix instruction
-    }
-#pragma unroll
-    for (int i = 0; i < kReads; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-      __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
   };
-  for (int s = 0; s < RING - 1; ++s) copy(ring + s * kStage);
+  auto next = [](int slot) { return slot == RING - 1 ? 0 : slot + 1; };
+  for (int s = 0; s <= RING - MEET; ++s, at = next(at)) {
+    clip();
+    copy(ring_to + s * kStage);
+  }
   Frag<T> fa[2][FM], fb[2][FN];
-  meet();  // stage 0
-  copy_read(ring + (RING - 1) * kStage, ring, fa[0], fb[0]);
-  int slot = 1;
+  meet(std::integral_constant<int, RING - MEET>{});  // stage 0
+  read(ring, fa[0], fb[0]);
+  int slot = 1 % RING;  // of the next stage to read
+  typedef std::integral_constant<int, RING - 2 * MEET> Under;
+  constexpr bool kPairs = sizeof(T) == 4;  // stages in pairs; one past the end holds zeros
+  Split sa[kPairs ? FM : 1], sb[kPairs ? FN : 1];
   if (w.m0 + w.wm < g.M && w.n0 + w.wn < g.N) {
     for (int s = 0; s < steps; s += 2) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (s + h < steps) {
-          meet();  // stage s + h + 1 is in LDS, the slot of stage s + h is free
-          copy_read(ring + (slot == 0 ? RING - 1 : slot - 1) * kStage, ring + slot * kStage, fa[1 - h], fb[1 - h]);
-          mma_all<T>(fa[h], fb[h], acc);
-          interleave();
-          slot = slot == RING - 1 ? 0 : slot + 1;
+        if (kPairs || s + h < steps) {
+          clip();
+          if (h % MEET == 0) meet(Under{});
+          copy_read(ring_to + at * kStage, ring + slot * kStage, fa[1 - h], fb[1 - h]);
+          if constexpr (kPairs) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) sb[j].take(fb[h][j].v, h);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+              sa[i].take(fa[h][i].v, h);
+              if (h == 1) mma_split(sa[i], sb, acc[i]);
+            }
+            if (h == 1) {  // the splitting of one fragment beside the products of the one before
+#pragma unroll
+              for (int i = 0; i < FM * FN * 6; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);  // vector arithmetic
+              }
+            }
+          } else {
+            mma_all<T>(fa[h], fb[h], acc);
+            interleave();
+          }
+          at = next(at);
+          slot = next(slot);
         }
       }
     }
   } else {  // a wave past the edge: its share of the copies only
-    for (int s = 0; s < steps; ++s) {
-      meet();
-      copy(ring + (slot == 0 ? RING - 1 : slot - 1) * kStage);
-      slot = slot == RING - 1 ? 0 : slot + 1;
+    for (int s = 0; s < steps + (kPairs ? steps % 2 : 0); ++s, at = next(at)) {
+      clip();
+      if (s % MEET == 0) meet(Under{});
+      copy(ring_to + at * kStage);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the stages
@@ -698,15 +793,15 @@ __global__ __launch_bounds__(kBlock) void align_rows_kernel(const Copy a, const 
 template <typename T, bool AK, bool BK>
 int launch_gemm_as(const Gemm &g, hipStream_t s) {
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-#define SFT_RING(BM, BN, WM, WN, RING)                                                                  \
-  hipLaunchKernelGGL((gemm_ring_kernel<T, AK, BK, BM, BN, WM, WN, RING>), dim3((unsigned)grid),         \
+#define SFT_RING(BM, BN, WM, WN, RING, MEET)                                                                  \
+  hipLaunchKernelGGL((gemm_ring_kernel<T, AK, BK, BM, BN, WM, WN, RING, MEET>), dim3((unsigned)grid),         \
                      dim3(WM *WN *kWave), 0, s, g)
   if (g.tile == kTile64) {
-    SFT_RING(64, 128, 2, 2, 4);
+    SFT_RING(64, 128, 2, 2, 4, 1);
   } else if (g.tile == kTile128) {
-    SFT_RING(128, 128, 2, 2, 3);
+    SFT_RING(128, 128, 2, 2, 3, 1);
   } else {
-    if constexpr (sizeof(T) == 2) SFT_RING(256, 256, 2, 4, 4);
+    if constexpr (sizeof(T) == 2) SFT_RING(256, 256, 2, 4, 4, 1);
   }
 #undef SFT_RING
   if (g.splits > 1) {

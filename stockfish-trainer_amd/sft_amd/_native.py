@@ -787,14 +787,18 @@ def type_code(dtype: torch.dtype) -> int:
     return code
 
 
+_get_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _call(name: str, device: torch.device, *args) -> None:
     """lib().name(*args, stream): on the tensors' device and its current stream."""
-    fn = getattr(_lib or lib(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    fn, index = getattr(_lib or lib(), name), device.index
+    if index == _get_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc != SFT_OK:
         _check(rc, name)
 
