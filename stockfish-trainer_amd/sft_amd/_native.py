@@ -9,6 +9,7 @@ tensor is not on a GPU, they raise.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -159,8 +160,12 @@ NOALLOC_SIGNATURES = {
         [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _u32, _vp]),
 }
 
+# The dense head's operators for eager torch programs (csrc/host/dense_binding.cpp).
+DENSE_BINDING_PATH = os.path.join(PKG_ROOT, "lib", "_sft_dense.so")
+
 _lib = None
 _noalloc_lib = None
+_dense_binding = None
 _lock = threading.Lock()
 
 
@@ -207,6 +212,23 @@ def noalloc_lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _noalloc_lib = handle
     return _noalloc_lib
+
+
+def dense_binding():
+    """The dense head's binding module; loads libsft_ft.so first, whose entry points it calls."""
+    global _dense_binding
+    if _dense_binding is None:
+        lib()
+        with _lock:
+            if _dense_binding is None:
+                if not os.path.exists(DENSE_BINDING_PATH):
+                    raise NativeLibraryMissing(
+                        f"{DENSE_BINDING_PATH} not found: build it with `make -C stockfish-trainer_amd/csrc`")
+                spec = importlib.util.spec_from_file_location("_sft_dense", DENSE_BINDING_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _dense_binding = module
+    return _dense_binding
 
 
 def last_error() -> str:
@@ -775,10 +797,7 @@ def quantize_i16(x: torch.Tensor, scale: float) -> torch.Tensor:
 
 
 # ---- the dense head ----
-# Small calls of these are bound by the host, so pointers and streams go as plain
-# integers and the device is set only where it is not the current one.
 _TYPES = {torch.float32: SFT_TYPE_F32, torch.float16: SFT_TYPE_F16, torch.bfloat16: SFT_TYPE_BF16}
-_SIZES = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
 
 
 def type_code(dtype: torch.dtype) -> int:
@@ -787,20 +806,10 @@ def type_code(dtype: torch.dtype) -> int:
     return code
 
 
-_get_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 def _call(name: str, device: torch.device, *args) -> None:
     """lib().name(*args, stream): on the tensors' device and its current stream."""
-    fn, index = getattr(_lib or lib(), name), device.index
-    if index == _get_device():
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(index))
-    if rc != SFT_OK:
-        _check(rc, name)
+    with torch.cuda.device(device):
+        _check(getattr(lib(), name)(*args, _stream(device)), name)
 
 
 def _at(t: torch.Tensor | None):
@@ -818,7 +827,7 @@ def _rows(t: torch.Tensor) -> int:
 def _copy_flag(*operands: torch.Tensor) -> int:
     """SFT_LINEAR_COPY if a dense-rows operand is not one that products read in place."""
     for t in operands:
-        stride = _rows(t) * _SIZES[t.dtype]
+        stride = _rows(t) * t.element_size()
         if (t.data_ptr() | stride) & 15 or stride > 1 << 23:
             return SFT_LINEAR_COPY
     return 0

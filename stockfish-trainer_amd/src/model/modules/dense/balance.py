@@ -21,17 +21,19 @@ from torch import Tensor, autograd
 
 from sft_amd import _native
 
-from .ops import calls
+from . import ops  # noqa: F401  (registers torch.ops.sft.*)
 from .rows import dense_rows
 
 
 class ExpertBalanceFunction(autograd.Function):
-    """apply(logits [T, E], mask [T] or None, top_k) -> (loss, counts)."""
+    """The operator in programs that are being compiled; eager ones record the binding's node.
+
+    apply(logits [T, E], mask [T] or None, top_k) -> (loss, counts)."""
 
     @staticmethod
     def forward(ctx, logits, mask, top_k):
         logits = dense_rows(logits)
-        loss, counts, kept = calls().balance_fwd(logits, mask, top_k)
+        loss, counts, kept = torch.ops.sft.balance_fwd(logits, mask, top_k)
         ctx.save_for_backward(logits, mask, counts, kept)
         ctx.top_k = top_k
         ctx.mark_non_differentiable(counts)
@@ -41,21 +43,13 @@ class ExpertBalanceFunction(autograd.Function):
     @autograd.function.once_differentiable
     def backward(ctx, grad_loss, _):
         logits, mask, counts, kept = ctx.saved_tensors
-        return calls().balance_bwd(logits, mask, ctx.top_k, counts, kept, grad_loss.float()), None, None
+        return torch.ops.sft.balance_bwd(logits, mask, ctx.top_k, counts, kept, grad_loss.float()), None, None
 
 
 def expert_balance(logits: Tensor, top_k: int = 1, mask: Tensor | None = None) -> tuple[Tensor, Tensor]:
     """(loss, a float32 scalar; counts, int64 [E]) of router logits [..., E] and a bool mask [...] of the
     positions that count (None: all)."""
-    assert logits.is_cuda and logits.dim() >= 1
-    assert logits.dtype in (torch.float32, torch.float16, torch.bfloat16)
-    E = logits.shape[-1]
-    assert 1 <= E <= _native.SFT_BALANCE_MAX_EXPERTS
-    assert 1 <= top_k <= E
-    if mask is not None:
-        assert mask.dtype == torch.bool and mask.device == logits.device
-        assert mask.shape == logits.shape[:-1]
-        mask = mask.reshape(-1).contiguous()
-    if logits.dim() != 2:
-        logits = logits.reshape(-1, E)
-    return ExpertBalanceFunction.apply(logits, mask, top_k)
+    if not torch.compiler.is_compiling():
+        return _native.dense_binding().balance(logits, top_k, mask)
+    mask = None if mask is None else mask.reshape(-1).contiguous()
+    return ExpertBalanceFunction.apply(logits.reshape(-1, logits.shape[-1]), mask, top_k)

@@ -19,64 +19,51 @@ know each row's weight in the total loss beforehand: logits.backward(grad).
 
 from __future__ import annotations
 
-import math
-
 import torch
 from torch import Tensor, autograd
 
 from sft_amd import _native
 
-from .ops import calls
+from . import ops  # noqa: F401  (registers torch.ops.sft.*)
 from .rows import dense_rows
 
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
-
-
 class DistillFunction(autograd.Function):
-    """apply(student [R, V], teacher [R, k], indices [R, k], temperature) -> loss [R]."""
+    """The operator in programs that are being compiled; eager ones record the binding's node.
+
+    apply(student [R, V], teacher [R, k], indices [R, k], temperature) -> loss [R]."""
 
     @staticmethod
     def forward(ctx, student, teacher, indices, temperature):
         ctx.save_for_backward(student, teacher, indices)
         ctx.temperature = temperature
-        return calls().distill_loss(student, teacher, indices, temperature)
+        return torch.ops.sft.distill_loss(student, teacher, indices, temperature)
 
     @staticmethod
     @autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         student, teacher, indices = ctx.saved_tensors
-        return calls().distill_grad(student, teacher, indices, ctx.temperature,
+        return torch.ops.sft.distill_grad(student, teacher, indices, ctx.temperature,
                                           grad_loss.float().contiguous()), None, None, None
-
-
-def _checked(student, teacher_logits, teacher_indices, temperature):
-    assert student.is_cuda and student.dim() == 2 and student.shape[1] >= 1
-    assert student.dtype in _FLOATS and teacher_logits.dtype in _FLOATS
-    assert teacher_indices.dtype in (torch.int32, torch.int64)
-    assert teacher_logits.dim() == 2 and teacher_logits.shape == teacher_indices.shape
-    assert teacher_logits.shape[0] == student.shape[0]
-    assert 1 <= teacher_logits.shape[1] <= _native.SFT_DISTILL_MAX_K
-    assert teacher_logits.device == student.device and teacher_indices.device == student.device
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
-    return dense_rows(student), teacher_logits.detach().contiguous(), teacher_indices.contiguous()
 
 
 def distill_loss(student_logits: Tensor, teacher_logits: Tensor, teacher_indices: Tensor,
                  temperature: float = 1.0) -> Tensor:
     """Per-row loss (float32 [R]) of student logits [R, V] against a teacher's k top logits [R, k] of the
     classes in teacher_indices (int32 or int64; outside [0, V): an empty slot)."""
-    student, teacher, indices = _checked(student_logits, teacher_logits, teacher_indices, temperature)
-    return DistillFunction.apply(student, teacher, indices, float(temperature))
+    if not torch.compiler.is_compiling():
+        return _native.dense_binding().distill_loss(student_logits, teacher_logits, teacher_indices, temperature)
+    return DistillFunction.apply(dense_rows(student_logits), teacher_logits.detach().contiguous(),
+                                 teacher_indices.contiguous(), float(temperature))
 
 
 def distill_loss_and_grad(student_logits: Tensor, teacher_logits: Tensor, teacher_indices: Tensor,
                           row_weight: Tensor | None = None, temperature: float = 1.0) -> tuple[Tensor, Tensor]:
     """(loss [R], row_weight * d loss / d student [R, V]) in one pass over the logits, outside autograd;
     row_weight float32 [R] (None: 1) is each row's share of the total loss, loss scaling included."""
-    student, teacher, indices = _checked(student_logits, teacher_logits, teacher_indices, temperature)
-    if row_weight is not None:
-        assert row_weight.shape == (student.shape[0],) and row_weight.dtype == torch.float32
-        assert row_weight.device == student.device
-        row_weight = row_weight.detach().contiguous()
-    return calls().distill_loss_and_grad(student.detach(), teacher, indices, float(temperature), row_weight)
+    if not torch.compiler.is_compiling():
+        return _native.dense_binding().distill_loss_and_grad(student_logits, teacher_logits, teacher_indices,
+                                                             row_weight, temperature)
+    row_weight = None if row_weight is None else row_weight.detach().contiguous()
+    return torch.ops.sft.distill_loss_and_grad(dense_rows(student_logits.detach()),
+                                               teacher_logits.detach().contiguous(), teacher_indices.contiguous(),
+                                               float(temperature), row_weight)

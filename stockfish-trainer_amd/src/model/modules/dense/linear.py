@@ -20,7 +20,7 @@ from torch import Tensor, autograd
 
 from sft_amd import _native
 
-from .ops import calls
+from . import ops  # noqa: F401  (registers torch.ops.sft.*)
 from .rows import dense_rows
 
 ACTIVATIONS = {
@@ -34,13 +34,15 @@ ACTIVATIONS = {
 
 
 class FusedLinearFunction(autograd.Function):
-    """apply(x [M, K], weight [N, K], bias [N] or None, residual [M, N] or None, act code) -> y [M, N]."""
+    """The operator in programs that are being compiled; eager ones record the binding's node.
+
+    apply(x [M, K], weight [N, K], bias [N] or None, residual [M, N] or None, act code) -> y [M, N]."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         x, weight, residual = dense_rows(x), dense_rows(weight), dense_rows(residual)
         bias = None if bias is None else bias.contiguous()
-        y, deriv = calls().linear_fwd(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        y, deriv = torch.ops.sft.linear_fwd(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, deriv)
         ctx.act = act
         return y
@@ -52,7 +54,7 @@ class FusedLinearFunction(autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            dx, dw, db = calls().linear_bwd(dense_rows(grad_y), deriv, x, weight, ctx.act, *need[:3])
+            dx, dw, db = torch.ops.sft.linear_bwd(dense_rows(grad_y), deriv, x, weight, ctx.act, *need[:3])
         return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None,
                 grad_y if need[3] else None, None)
 
@@ -63,27 +65,10 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-    assert weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1]
+    if not torch.compiler.is_compiling():
+        return _native.dense_binding().linear(x, weight, bias, residual, act)
     N, K = weight.shape
-    assert N > 0 and K > 0
     lead = x.shape[:-1]
-    dtype, device = x.dtype, x.device
-    assert x.is_cuda and dtype in (torch.float32, torch.float16, torch.bfloat16)
-    for t in (weight, bias, residual):
-        if t is not None:
-            assert t.device == device and t.dtype == dtype
-    if bias is not None:
-        assert bias.shape == (N,)
-    if residual is not None:
-        assert residual.shape == (*lead, N)
-    if x.dim() != 2:
-        x = x.reshape(-1, K)
-        residual = None if residual is None else residual.reshape(-1, N)
-    if torch.is_grad_enabled() or torch.compiler.is_compiling():
-        y = FusedLinearFunction.apply(x, weight, bias, residual, act)
-    else:
-        # nothing to record: straight to the library
-        x, weight, residual = dense_rows(x), dense_rows(weight), dense_rows(residual)
-        y = torch.empty(x.shape[0], N, dtype=dtype, device=device)
-        _native.linear_fwd(x, weight, None if bias is None else bias.contiguous(), residual, y, None, act)
-    return y if len(lead) == 1 else y.view(*lead, N)
+    x = x.reshape(-1, K)
+    residual = None if residual is None else residual.reshape(-1, N)
+    return FusedLinearFunction.apply(x, weight, bias, residual, act).view(*lead, N)

@@ -1,8 +1,9 @@
-"""The dense head's library calls, and the same as torch custom operators: opaque
-to Dynamo and Inductor, with known output shapes, as the feature transformer's
-are.  Every call allocates and returns its outputs and mutates nothing.  Eager
-programs take the plain functions (`eager` below): a custom operator's dispatch
-costs more than a small call's kernels.
+"""The dense head's library calls as torch custom operators, for programs that are
+being compiled: opaque to Dynamo and Inductor, with known output shapes, as the
+feature transformer's are.  Every op allocates and returns its outputs and mutates
+nothing.  Eager programs take the same calls through the binding module
+(sft_amd/_native.py, dense_binding), whose dispatch costs less than a small
+call's kernels.
 """
 
 from __future__ import annotations
@@ -17,8 +18,10 @@ def _deriv_dtype(dtype: torch.dtype) -> torch.dtype:
     return torch.float32 if dtype == torch.float32 else torch.int16
 
 
-def _linear_fwd(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, act: int,
-                keep: bool) -> tuple[Tensor, Tensor]:
+# ---- FusedLinearFunction ----
+@torch.library.custom_op("sft::linear_fwd", mutates_args=(), device_types="cuda")
+def linear_fwd(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, act: int,
+               keep: bool) -> tuple[Tensor, Tensor]:
     """(y, act' of every output for the backward; empty where it is not kept or is 1)."""
     M, N = x.shape[0], weight.shape[0]
     y = torch.empty(M, N, dtype=x.dtype, device=x.device)
@@ -28,89 +31,23 @@ def _linear_fwd(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor
     return y, deriv
 
 
-def _linear_bwd(grad_y: Tensor, deriv: Tensor, x: Tensor, weight: Tensor, act: int, need_x: bool, need_weight: bool,
-                need_bias: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """Grads of x, weight and bias; empty where not needed."""
-    (M, K), N = x.shape, weight.shape[0]
-    dx = torch.empty((M, K) if need_x else (0,), dtype=x.dtype, device=x.device)
-    dw = torch.empty((N, K) if need_weight else (0,), dtype=x.dtype, device=x.device)
-    db = torch.empty((N,) if need_bias else (0,), dtype=x.dtype, device=x.device)
-    _native.linear_bwd(grad_y, None if act == _native.SFT_ACT_NONE else deriv, x, weight, dx if need_x else None,
-                       dw if need_weight else None, db if need_bias else None, act)
-    return dx, dw, db
-
-
-def _balance_fwd(logits: Tensor, mask: Tensor | None, top_k: int) -> tuple[Tensor, Tensor, Tensor]:
-    """(loss, counts [E], number of kept positions)."""
-    loss = torch.empty((), dtype=torch.float32, device=logits.device)
-    counts = torch.empty(logits.shape[1], dtype=torch.int64, device=logits.device)
-    kept = torch.empty((), dtype=torch.int64, device=logits.device)
-    _native.balance_fwd(logits, mask, top_k, loss, counts, kept)
-    return loss, counts, kept
-
-
-def _balance_bwd(logits: Tensor, mask: Tensor | None, top_k: int, counts: Tensor, kept: Tensor,
-                 grad_loss: Tensor) -> Tensor:
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _native.balance_bwd(logits, mask, top_k, counts, kept, grad_loss, grad)
-    return grad
-
-
-def _distill_loss(student: Tensor, teacher: Tensor, indices: Tensor, temperature: float) -> Tensor:
-    loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device)
-    _native.distill(student, teacher, indices, temperature, None, loss, None)
-    return loss
-
-
-def _distill_grad(student: Tensor, teacher: Tensor, indices: Tensor, temperature: float, row_weight: Tensor) -> Tensor:
-    grad = torch.empty(student.shape, dtype=student.dtype, device=student.device)
-    _native.distill(student, teacher, indices, temperature, row_weight, None, grad)
-    return grad
-
-
-def _distill_loss_and_grad(student: Tensor, teacher: Tensor, indices: Tensor, temperature: float,
-                           row_weight: Tensor | None) -> tuple[Tensor, Tensor]:
-    loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device)
-    grad = torch.empty(student.shape, dtype=student.dtype, device=student.device)
-    _native.distill(student, teacher, indices, temperature, row_weight, loss, grad)
-    return loss, grad
-
-
-class eager:
-    """The calls without a custom operator's dispatch."""
-
-    linear_fwd = staticmethod(_linear_fwd)
-    linear_bwd = staticmethod(_linear_bwd)
-    balance_fwd = staticmethod(_balance_fwd)
-    balance_bwd = staticmethod(_balance_bwd)
-    distill_loss = staticmethod(_distill_loss)
-    distill_grad = staticmethod(_distill_grad)
-    distill_loss_and_grad = staticmethod(_distill_loss_and_grad)
-
-
-def calls():
-    """torch.ops.sft while a program is being compiled, else `eager`."""
-    return torch.ops.sft if torch.compiler.is_compiling() else eager
-
-
-def _op(name, fn):
-    return torch.library.custom_op(f"sft::{name}", fn, mutates_args=(), device_types="cuda")
-
-
-linear_fwd = _op("linear_fwd", _linear_fwd)
-linear_bwd = _op("linear_bwd", _linear_bwd)
-balance_fwd = _op("balance_fwd", _balance_fwd)
-balance_bwd = _op("balance_bwd", _balance_bwd)
-distill_loss = _op("distill_loss", _distill_loss)
-distill_grad = _op("distill_grad", _distill_grad)
-distill_loss_and_grad = _op("distill_loss_and_grad", _distill_loss_and_grad)
-
-
 @linear_fwd.register_fake
 def _(x, weight, bias, residual, act, keep):
     shape = (x.shape[0], weight.shape[0])
     kept = keep and act != _native.SFT_ACT_NONE
     return x.new_empty(shape), x.new_empty(shape if kept else (0,), dtype=_deriv_dtype(x.dtype))
+
+
+@torch.library.custom_op("sft::linear_bwd", mutates_args=(), device_types="cuda")
+def linear_bwd(grad_y: Tensor, deriv: Tensor, x: Tensor, weight: Tensor, act: int, need_x: bool, need_weight: bool,
+               need_bias: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """Grads of x, weight and bias; empty where not needed."""
+    (M, K), N = x.shape, weight.shape[0]
+    dx, dw, db = (torch.empty(shape if need else (0,), dtype=x.dtype, device=x.device)
+                  for need, shape in ((need_x, (M, K)), (need_weight, (N, K)), (need_bias, (N,))))
+    _native.linear_bwd(grad_y, None if act == _native.SFT_ACT_NONE else deriv, x, weight, dx if need_x else None,
+                       dw if need_weight else None, db if need_bias else None, act)
+    return dx, dw, db
 
 
 @linear_bwd.register_fake
@@ -120,10 +57,29 @@ def _(grad_y, deriv, x, weight, act, need_x, need_weight, need_bias):
                  for need, shape in ((need_x, (M, K)), (need_weight, (N, K)), (need_bias, (N,))))
 
 
+# ---- ExpertBalanceFunction ----
+@torch.library.custom_op("sft::balance_fwd", mutates_args=(), device_types="cuda")
+def balance_fwd(logits: Tensor, mask: Tensor | None, top_k: int) -> tuple[Tensor, Tensor, Tensor]:
+    """(loss, counts [E], number of kept positions)."""
+    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    counts = torch.empty(logits.shape[1], dtype=torch.int64, device=logits.device)
+    kept = torch.empty((), dtype=torch.int64, device=logits.device)
+    _native.balance_fwd(logits, mask, top_k, loss, counts, kept)
+    return loss, counts, kept
+
+
 @balance_fwd.register_fake
 def _(logits, mask, top_k):
     return (logits.new_empty((), dtype=torch.float32), logits.new_empty((logits.shape[1],), dtype=torch.int64),
             logits.new_empty((), dtype=torch.int64))
+
+
+@torch.library.custom_op("sft::balance_bwd", mutates_args=(), device_types="cuda")
+def balance_bwd(logits: Tensor, mask: Tensor | None, top_k: int, counts: Tensor, kept: Tensor,
+                grad_loss: Tensor) -> Tensor:
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _native.balance_bwd(logits, mask, top_k, counts, kept, grad_loss, grad)
+    return grad
 
 
 @balance_bwd.register_fake
@@ -131,14 +87,38 @@ def _(logits, mask, top_k, counts, kept, grad_loss):
     return logits.new_empty(logits.shape)
 
 
+# ---- DistillFunction ----
+@torch.library.custom_op("sft::distill_loss", mutates_args=(), device_types="cuda")
+def distill_loss(student: Tensor, teacher: Tensor, indices: Tensor, temperature: float) -> Tensor:
+    loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device)
+    _native.distill(student, teacher, indices, temperature, None, loss, None)
+    return loss
+
+
 @distill_loss.register_fake
 def _(student, teacher, indices, temperature):
     return student.new_empty((student.shape[0],), dtype=torch.float32)
 
 
+@torch.library.custom_op("sft::distill_grad", mutates_args=(), device_types="cuda")
+def distill_grad(student: Tensor, teacher: Tensor, indices: Tensor, temperature: float, row_weight: Tensor) -> Tensor:
+    grad = torch.empty(student.shape, dtype=student.dtype, device=student.device)
+    _native.distill(student, teacher, indices, temperature, row_weight, None, grad)
+    return grad
+
+
 @distill_grad.register_fake
 def _(student, teacher, indices, temperature, row_weight):
     return student.new_empty(student.shape)
+
+
+@torch.library.custom_op("sft::distill_loss_and_grad", mutates_args=(), device_types="cuda")
+def distill_loss_and_grad(student: Tensor, teacher: Tensor, indices: Tensor, temperature: float,
+                          row_weight: Tensor | None) -> tuple[Tensor, Tensor]:
+    loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device)
+    grad = torch.empty(student.shape, dtype=student.dtype, device=student.device)
+    _native.distill(student, teacher, indices, temperature, row_weight, loss, grad)
+    return loss, grad
 
 
 @distill_loss_and_grad.register_fake
