@@ -97,7 +97,7 @@ struct Deriv<float> {
   static __device__ __forceinline__ float unpack(float d) { return d; }
 };
 
-// V consecutive elements: in one access, or element by element the first `cnt`.
+// V consecutive elements in one access, or the first `cnt` one by one.
 template <typename T, int V>
 __device__ __forceinline__ void load_v(const T *p, bool vec, int cnt, T (&v)[V]) {
   if (vec) {
@@ -121,11 +121,11 @@ __device__ __forceinline__ void store_v(T *p, bool vec, int cnt, const T (&v)[V]
 // y[m, n..n+V-1] = residual + act(z + bias), rounded once; the derivative beside it.
 // Called only with m < M and n < N.
 template <typename T, int V>
-__device__ __forceinline__ void finish(const Epilogue &e, int64_t m, int n, int N, float (&z)[V]) {
+__device__ __forceinline__ void finish(const Epilogue &e, int64_t m, int n, int N, float (&z)[V], bool vec) {
   const int cnt = N - n;
   if (e.bias) {
     T b[V];
-    load_v(static_cast<const T *>(e.bias) + n, e.vec, cnt, b);
+    load_v(static_cast<const T *>(e.bias) + n, vec, cnt, b);
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] += (float)b[i];
   }
@@ -137,19 +137,19 @@ __device__ __forceinline__ void finish(const Epilogue &e, int64_t m, int n, int 
       D q[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) q[i] = Deriv<T>::pack(d[i]);
-      store_v(static_cast<D *>(e.deriv) + m * N + n, e.vec, cnt, q);
+      store_v(static_cast<D *>(e.deriv) + m * N + n, vec, cnt, q);
     }
   }
   if (e.residual) {
     T r[V];
-    load_v(static_cast<const T *>(e.residual) + m * e.ldr + n, e.vec, cnt, r);
+    load_v(static_cast<const T *>(e.residual) + m * e.ldr + n, vec, cnt, r);
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] += (float)r[i];
   }
   T y[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) y[i] = (T)z[i];
-  store_v(static_cast<T *>(e.y) + m * e.ldy + n, e.vec, cnt, y);
+  store_v(static_cast<T *>(e.y) + m * e.ldy + n, vec, cnt, y);
 }
 
 // ---- tiles in LDS ----
@@ -437,42 +437,48 @@ struct TileWork {
     wn = (wave % WN) * (BN / WN);
   }
   // The first operand's rows are the result's four registers: lane l holds m = l % 16
-  // and n = 4 (l / 16) + 0..3 of each fragment.  A wave turns its sums in LDS, a part
-  // of the rows at a time, so that its lanes take whole vectors of a row: memory sees
-  // full lines, and the epilogue's code is there once per part.
+  // and n = 4 (l / 16) + 0..3 of each fragment.  A wave turns its sums in LDS, 32 rows
+  // at a time, so that its lanes take whole vectors of a row (single elements where
+  // rows are not made of them): memory sees full lines, and the epilogue's code is
+  // there once per part.
   static constexpr int kWaveN = BN / WN, kPitch = kWaveN + 4;  // floats; 4 spread the rows over the banks
-  static constexpr int kParts = FM / 2;  // 32 rows
-  static constexpr int kPartM = FM / kParts;
-  static constexpr int kTurnBytes = kPartM * 16 * kPitch * 4 * WM * WN;
-  __device__ __forceinline__ void finish_all(const Gemm &g, const f32x4 (&acc)[FM][FN], char *lds) const {
-    constexpr int V = 16 / (int)sizeof(T), kLanes = kWaveN / V, kRows = kWave / kLanes;
+  static constexpr int kParts = FM / 2, kPartRows = 32;
+  static constexpr int kTurnBytes = kPartRows * kPitch * 4 * WM * WN;
+  template <int V>
+  __device__ __forceinline__ void finish_part(const Gemm &g, int m1, const float *turn) const {
+    constexpr int kLanes = kWaveN / V, kRows = kWave / kLanes;
     const int lane = lane_id();
-    float *turn = reinterpret_cast<float *>(lds) + (threadIdx.x / kWave) * (kPartM * 16 * kPitch);
-    const int n = n0 + wn + lane % kLanes * V;
+    const int c = lane % kLanes * V, n = n0 + wn + c;
+    const int rows = n < g.N ? (g.M - m1 < kPartRows ? g.M - m1 : kPartRows) : 0;
+#pragma unroll 2
+    for (int r = lane / kLanes; r < rows; r += kRows) {
+      float z[V];
+      __builtin_memcpy(z, __builtin_assume_aligned(turn + r * kPitch + c, 4 * (V < 4 ? V : 4)), 4 * V);
+      if (g.part)
+        store_v(g.part + ((int64_t)split * g.M + m1 + r) * g.N + n, true, V, z);
+      else
+        finish<T>(g.epi, m1 + r, n, g.N, z, true);
+    }
+  }
+  __device__ __forceinline__ void finish_all(const Gemm &g, const f32x4 (&acc)[FM][FN], char *lds) const {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int lane = lane_id();
+    float *turn = reinterpret_cast<float *>(lds) + (threadIdx.x / kWave) * (kPartRows * kPitch);
+    const bool wide = g.part ? g.N % V == 0 : g.epi.vec;
     __syncthreads();  // every wave has done with the stages
 #pragma unroll
     for (int part = 0; part < kParts; ++part) {
 #pragma unroll
-      for (int i = 0; i < kPartM; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
           *reinterpret_cast<f32x4 *>(turn + (i * 16 + lane % 16) * kPitch + j * 16 + lane / 16 * 4) =
-              acc[part * kPartM + i][j];
+              acc[part * 2 + i][j];
       wave_lds_barrier();
-#pragma unroll 1
-      for (int r = lane / kLanes; r < kPartM * 16; r += kRows) {
-        const int m = m0 + wm + part * kPartM * 16 + r;
-        if (m >= g.M || n >= g.N) break;
-        float z[V];
-#pragma unroll
-        for (int i = 0; i < V; i += 4)
-          *reinterpret_cast<f32x4 *>(z + i) =
-              *reinterpret_cast<const f32x4 *>(turn + r * kPitch + lane % kLanes * V + i);
-        if (g.part)
-          store_v(g.part + ((int64_t)split * g.M + m) * g.N + n, g.N % V == 0, g.N - n, z);
-        else
-          finish<T>(g.epi, m, n, g.N, z);
-      }
+      if (wide)
+        finish_part<V>(g, m0 + wm + part * kPartRows, turn);
+      else
+        finish_part<1>(g, m0 + wm + part * kPartRows, turn);
       wave_lds_barrier();
     }
   }
@@ -615,24 +621,24 @@ __global__ __launch_bounds__(WM *WN *kWave, BM / WM * BN / WN > 128 * 64 ? 1 : 2
   w.finish_all(g, acc, lds);
 }
 
-// Sums a split product's partials in split order and finishes them.
-template <typename T>
+// Sums a split product's partials in split order and finishes them; V elements a thread.
+template <typename T, int V>
 __global__ __launch_bounds__(kBlock) void gemm_join_kernel(const Gemm g) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int64_t vecs = (g.N + V - 1) / V;
+  const int64_t vecs = g.N / V;  // N is a multiple of V
   const int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x;
   if (q >= vecs * g.M) return;
   const int64_t m = q / vecs;
   const int n = (int)(q % vecs) * V;
   float z[V] = {};
   const float *p = g.part + m * g.N + n;
+#pragma unroll 8
   for (int s = 0; s < g.splits; ++s, p += (int64_t)g.M * g.N) {
     float v[V];
-    load_v(p, g.N % V == 0, g.N - n, v);
+    load_v(p, true, V, v);
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] += v[i];
   }
-  finish<T>(g.epi, m, n, g.N, z);
+  finish<T>(g.epi, m, n, g.N, z, true);
 }
 
 // ---- few rows ----
@@ -699,7 +705,7 @@ __global__ __launch_bounds__(kRowWaves *kWave) void gemm_rows_kernel(const Gemm 
   for (int s = 1; s < kRowWaves; ++s) sum += red[s][f][lane];
   const int m = f * 16 + i, n = n0 + c * 4;
   float z[4] = {sum.x, sum.y, sum.z, sum.w};
-  if (m < g.M && n < g.N) finish<T>(g.epi, m, n, g.N, z);
+  if (m < g.M && n < g.N) finish<T>(g.epi, m, n, g.N, z, g.epi.vec);
 }
 
 // ---- gradient of the activation, and the bias grad's partial sums ----
@@ -766,8 +772,10 @@ __global__ __launch_bounds__(kJoinCols *kJoinRows) void bias_join_kernel(const f
   const int c = threadIdx.x % kJoinCols, r = threadIdx.x / kJoinCols;
   const int n = blockIdx.x * kJoinCols + c;
   float s = 0.f;
-  if (n < N)
+  if (n < N) {
+#pragma unroll 8
     for (int i = r; i < parts; i += kJoinRows) s += part[(int64_t)i * N + n];
+  }
   red[r][c] = s;
   __syncthreads();
   if (r != 0 || n >= N) return;
@@ -805,8 +813,13 @@ int launch_gemm_as(const Gemm &g, hipStream_t s) {
   }
 #undef SFT_RING
   if (g.splits > 1) {
-    const int64_t vecs = ceil_div(g.N, 16 / (int64_t)sizeof(T)) * g.M;
-    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)ceil_div(vecs, kBlock)), dim3(kBlock), 0, s, g);
+    constexpr int V = 16 / (int)sizeof(T);
+    const dim3 block(kBlock);
+    const int64_t n = (int64_t)g.N * g.M;
+    if (g.epi.vec)
+      hipLaunchKernelGGL((gemm_join_kernel<T, V>), dim3((unsigned)ceil_div(n / V, kBlock)), block, 0, s, g);
+    else
+      hipLaunchKernelGGL((gemm_join_kernel<T, 1>), dim3((unsigned)ceil_div(n, kBlock)), block, 0, s, g);
   }
   return check_launch("dense product");
 }
