@@ -27,7 +27,7 @@ using dense::group_reduce;
 using dense::group_sum;
 
 constexpr int kThreads = 1024;   // of the forward: 16 waves, whose sums leave as one partial
-constexpr int kMaxParts = 256;  // its workgroups, one per CU
+constexpr int kMaxParts = 512;  // its workgroups, two per CU
 
 // A row's logits: lane t of the group holds the chunks t + G j of V elements.  Loads
 // have no branches (whole: E is a multiple of V), so that the next row's are under way
@@ -70,7 +70,7 @@ struct Row {
     for (int j = 0; j < C; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        p[j][i] = expf(x[j][i] - m);
+        p[j][i] = __builtin_amdgcn_exp2f((x[j][i] - m) * 1.44269504088896341f);
         s += p[j][i];
       }
     const float r = 1.f / group_sum<G>(s);
@@ -145,19 +145,14 @@ __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restri
                                                                int64_t *counts, int64_t *kept_rows) {
   constexpr int V = Row<T, G, C, WHOLE>::V, kRows = kThreads / G, kWaves = kThreads / kWave;
   __shared__ float red_p[kWaves][G * C * V];
-  __shared__ int32_t red_c[kWaves][G * C * V];
+  __shared__ int32_t chosen[G * C * V];  // whole numbers: the order of adding does not matter
   __shared__ int32_t red_n[kWaves];
   const int lane = lane_id(), t = lane % G, wave = uniform(threadIdx.x / kWave);
   const uint64_t group = (G == kWave ? ~0ull : ((1ull << (G % kWave)) - 1)) << (lane / G * G);
-  float sum[C][V];
-  int32_t cnt[C][V], kept = 0;
-#pragma unroll
-  for (int j = 0; j < C; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      sum[j][i] = 0.f;
-      cnt[j][i] = 0;
-    }
+  float sum[C][V] = {};
+  int32_t kept = 0;
+  for (int e = threadIdx.x; e < G * C * V; e += kThreads) chosen[e] = 0;
+  __syncthreads();
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
   Row<T, G, C, WHOLE> row;
@@ -197,11 +192,11 @@ __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restri
         for (int i = V - 1; i >= 0; --i) first = row.x[j][i] == best ? i : first;
         const uint64_t hits = ballot(open && first < V) & group;
         const bool mine = hits && lane == __builtin_ctzll(hits);
+        if (mine) atomicAdd(&chosen[(t + G * j) * V + first], 1);
+        if (k + 1 < top_k) {
+          const int taken = mine ? first : V;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const bool at = mine && i == first;
-          cnt[j][i] += at;
-          row.x[j][i] = at ? -INFINITY : row.x[j][i];
+          for (int i = 0; i < V; ++i) row.x[j][i] = i == taken ? -INFINITY : row.x[j][i];
         }
         open = open && !hits;
       }
@@ -216,28 +211,18 @@ __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restri
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
-      for (int m = G; m < kWave; m <<= 1) {
-        sum[j][i] += __shfl_xor(sum[j][i], m);
-        cnt[j][i] += __shfl_xor(cnt[j][i], m);
-      }
-      if (lane < G) {
-        red_p[wave][(t + G * j) * V + i] = sum[j][i];
-        red_c[wave][(t + G * j) * V + i] = cnt[j][i];
-      }
+      for (int m = G; m < kWave; m <<= 1) sum[j][i] += __shfl_xor(sum[j][i], m);
+      if (lane < G) red_p[wave][(t + G * j) * V + i] = sum[j][i];
     }
   kept = group_reduce<kWave>(kept, add);
   if (lane == 0) red_n[wave] = kept;
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kThreads) {
     float p = red_p[0][e];
-    int32_t c = red_c[0][e];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      p += red_p[w][e];
-      c += red_c[w][e];
-    }
+    for (int w = 1; w < kWaves; ++w) p += red_p[w][e];
     part_p[(int64_t)blockIdx.x * E + e] = p;
-    part_c[(int64_t)blockIdx.x * E + e] = c;
+    part_c[(int64_t)blockIdx.x * E + e] = chosen[e];
   }
   if (threadIdx.x == 0) {
     int32_t n = 0;
