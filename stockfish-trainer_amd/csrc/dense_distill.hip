@@ -162,6 +162,8 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
   __shared__ float top[kWaves], sums[kWaves];
   __shared__ float shared_cross;
   __shared__ int shared_any;
+  __shared__ int slot_idx[kWaves > 1 ? SFT_DISTILL_MAX_K : 1];  // the teacher's side, until the end
+  __shared__ float slot_q[kWaves > 1 ? SFT_DISTILL_MAX_K : 1];
   const int tid = threadIdx.x % TPR, wave = uniform(tid / kWave);
   const int64_t row = (int64_t)blockIdx.x * kRowsPer + uniform(threadIdx.x / TPR);
   if (row >= d.rows) return;  // whole waves, and never part of a row's
@@ -193,7 +195,16 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
   float x_edge = (float)s[tid < edge ? mine : 0];
   if (tid >= edge) x_edge = -INFINITY;
   Teacher te;
-  if (wave == 0) te.load(d, row, s);
+  if (wave == 0) {
+    te.load(d, row, s);
+    if (kWaves > 1) {
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) {
+        slot_idx[lane_id() + j * kWave] = te.idx[j];
+        slot_q[lane_id() + j * kWave] = te.q[j];
+      }
+    }
+  }
   Running run;
   if (C) {
 #pragma unroll
@@ -269,6 +280,13 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if (kWaves > 1) __syncthreads();
   if (wave != 0) return;
+  if (kWaves > 1) {
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      te.idx[j] = slot_idx[lane_id() + j * kWave];
+      te.q[j] = slot_q[lane_id() + j * kWave];
+    }
+  }
   float total[kSlots];
   te.merged(d.k, total);
 #pragma unroll
@@ -295,7 +313,10 @@ void launch(const Distill &d, hipStream_t s) {
   SFT_DISTILL(1024, 256, 4)
   SFT_DISTILL(2048, 256, 8)
   SFT_DISTILL(4096, 1024, 4)
+  SFT_DISTILL(6144, 1024, 6)
   SFT_DISTILL(8192, 1024, 8)
+  SFT_DISTILL(10240, 1024, 10)
+  SFT_DISTILL(13312, 1024, 13)
   SFT_DISTILL(16384, 1024, 16)
   SFT_DISTILL(INT64_MAX, 1024, 0)
 #undef SFT_DISTILL
