@@ -19,7 +19,8 @@ struct Epilogue {
   void *deriv;           // dense [M, N] of act', or null
   int64_t ldr, ldy;
   int act;
-  bool vec;  // bias, residual, y and deriv take 16-byte accesses (of few rows: of 4 elements)
+  bool vec;     // bias, residual, y and deriv take 16-byte accesses (of few rows: of 4 elements)
+  bool stream;  // y goes past the caches
 };
 
 // C[M, N] = sum over K of A(m, k) B(n, k).  Operands padded to whole chunks have ma >= M

@@ -36,7 +36,7 @@ struct TileCost {
   int rows, cols, slots;              // slots: workgroups the card holds at once
   double stage[2], alone[2], round;   // us a stage of 16-bit types and of binary32, with many and one per CU
 };
-constexpr TileCost kTiles[3] = {{64, 128, 768, {0.17, 0.42}, {0.26, 0.58}, 4.0},
+constexpr TileCost kTiles[3] = {{64, 128, 768, {0.22, 0.42}, {0.32, 0.58}, 4.0},
                                 {128, 128, 768, {0.29, 0.70}, {0.42, 0.60}, 5.0},
                                 {256, 256, 256, {0.84, 0.0}, {0.84, 0.0}, 8.0}};
 Cut cut_of(int dtype, int64_t M, int64_t N, int64_t K) {
@@ -132,6 +132,10 @@ int run_gemm(int dtype, int layout, const Matrix &a, const Matrix &b, int64_t M,
   if (g.K < g.kb) g.K = g.kb;
   g.epi = epi;
   g.epi.vec = epilogue_vec(epi, N, es, 16 / es);
+  // Results past the caches, where a product's arithmetic takes longer than its stores:
+  // they leave the operands their room.  65536 x 1040 x 4096 bf16 622 -> 561 us, 16384 x
+  // 1040 x 1040 64 -> 59; with 4 stages (65536 x 1040 from 128) 46 -> 61.
+  g.epi.stream = g.epi.vec && K * es >= 16 * kStage;
   const Cut c = cut_of(dtype, M, N, K);
   g.tile = c.tile;
   g.tiles_m = c.tiles_m;
@@ -184,7 +188,7 @@ size_t linear_fwd_workspace(int dtype, const void *x, int64_t ldx, const void *w
 int linear_fwd(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
                const void *residual, int64_t ldr, void *y, int64_t ldy, void *deriv, int64_t M, int64_t K, int64_t N,
                int act, void *workspace, hipStream_t s) {
-  Epilogue epi{bias, residual, y, act == SFT_ACT_NONE ? nullptr : deriv, ldr, ldy, act, false};
+  Epilogue epi{bias, residual, y, act == SFT_ACT_NONE ? nullptr : deriv, ldr, ldy, act, false, false};
   if (M <= kRowsMost) {
     Gemm g = {};
     g.a = x;
@@ -253,10 +257,10 @@ int linear_bwd(int dtype, const void *dy, int64_t lddy, const void *deriv, const
   if (!rc) rc = align(dtype, dx ? &weight : nullptr, dw ? &in : nullptr, ws, s);
   if (!rc && dx)
     rc = run_gemm(dtype, kInputGrad, dz, weight, M, K, N,
-                  Epilogue{nullptr, nullptr, dx, nullptr, 0, K, SFT_ACT_NONE, false}, ws, s);
+                  Epilogue{nullptr, nullptr, dx, nullptr, 0, K, SFT_ACT_NONE, false, false}, ws, s);
   if (!rc && dw)
     rc = run_gemm(dtype, kWeightGrad, dz, in, N, K, M,
-                  Epilogue{nullptr, nullptr, dw, nullptr, 0, K, SFT_ACT_NONE, false}, ws, s);
+                  Epilogue{nullptr, nullptr, dw, nullptr, 0, K, SFT_ACT_NONE, false, false}, ws, s);
   return rc;
 }
 

@@ -26,6 +26,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 #define SFT_LDS __attribute__((address_space(3)))
 
+constexpr float kLog2E = 1.44269504088896341f;
 constexpr int kStageBytes = 64;  // bytes of k per tile row and pipeline stage: one fragment's
 
 // ---- activations ----
@@ -51,10 +52,12 @@ __device__ __forceinline__ void activate(float (&z)[V], float (&d)[V], int act) 
         z[i] = act == SFT_ACT_CRELU ? c : c * c;
       }
       break;
+    // Base-2 exponentials and reciprocals of the hardware, each within a unit in the
+    // last place or so.
     case SFT_ACT_SILU:
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float s = 1.f / (1.f + expf(-z[i]));
+        const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2E * z[i]));
         d[i] = s * (1.f + z[i] * (1.f - s));
         z[i] *= s;
       }
@@ -64,7 +67,8 @@ __device__ __forceinline__ void activate(float (&z)[V], float (&d)[V], int act) 
       // 1.5e-7; its exponential is the derivative's too.
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float a = fabsf(z[i]) * 0.70710678118654752f, e = expf(-a * a), t = 1.f / (1.f + 0.3275911f * a);
+        const float a = fabsf(z[i]) * 0.70710678118654752f, e = __builtin_amdgcn_exp2f(-kLog2E * a * a);
+        const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * a);
         const float tail =
             0.5f * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * e;
         const float cdf = z[i] < 0.f ? tail : 1.f - tail;
@@ -118,17 +122,23 @@ __device__ __forceinline__ void store_v(T *p, bool vec, int cnt, const T (&v)[V]
   }
 }
 
-// y[m, n..n+V-1] = residual + act(z + bias), rounded once; the derivative beside it.
-// Called only with m < M and n < N.
+// The bias of V columns (0 without one).
 template <typename T, int V>
-__device__ __forceinline__ void finish(const Epilogue &e, int64_t m, int n, int N, float (&z)[V], bool vec) {
-  const int cnt = N - n;
-  if (e.bias) {
-    T b[V];
-    load_v(static_cast<const T *>(e.bias) + n, vec, cnt, b);
+__device__ __forceinline__ void load_bias(const Epilogue &e, int n, int N, bool vec, float (&b)[V]) {
+  T v[V] = {};
+  if (e.bias) load_v(static_cast<const T *>(e.bias) + n, vec, N - n, v);
 #pragma unroll
-    for (int i = 0; i < V; ++i) z[i] += (float)b[i];
-  }
+  for (int i = 0; i < V; ++i) b[i] = (float)v[i];
+}
+
+// y[m, n..n+V-1] = residual + act(z + bias), rounded once; the derivative beside it.
+// Called only with m < M and n < N.  STREAM: y past the caches, in whole 16 bytes.
+template <typename T, bool STREAM, int V>
+__device__ __forceinline__ void finish(const Epilogue &e, int64_t m, int n, int N, const float (&bias)[V], float (&z)[V],
+                                       bool vec) {
+  const int cnt = N - n;
+#pragma unroll
+  for (int i = 0; i < V; ++i) z[i] += bias[i];
   if (e.act != SFT_ACT_NONE) {
     float d[V];
     activate(z, d, e.act);
@@ -149,7 +159,14 @@ __device__ __forceinline__ void finish(const Epilogue &e, int64_t m, int n, int 
   T y[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) y[i] = (T)z[i];
-  store_v(static_cast<T *>(e.y) + m * e.ldy + n, vec, cnt, y);
+  T *to = static_cast<T *>(e.y) + m * e.ldy + n;
+  if constexpr (STREAM) {
+    u32x4 q;
+    __builtin_memcpy(&q, y, 16);
+    __builtin_nontemporal_store(q, reinterpret_cast<u32x4 *>(to));
+    return;
+  }
+  store_v(to, vec, cnt, y);
 }
 
 // ---- tiles in LDS ----
@@ -444,12 +461,14 @@ struct TileWork {
   static constexpr int kWaveN = BN / WN, kPitch = kWaveN + 4;  // floats; 4 spread the rows over the banks
   static constexpr int kParts = FM / 2, kPartRows = 32;
   static constexpr int kTurnBytes = kPartRows * kPitch * 4 * WM * WN;
-  template <int V>
+  template <int V, bool STREAM>
   __device__ __forceinline__ void finish_part(const Gemm &g, int m1, const float *turn) const {
     constexpr int kLanes = kWaveN / V, kRows = kWave / kLanes;
     const int lane = lane_id();
     const int c = lane % kLanes * V, n = n0 + wn + c;
     const int rows = n < g.N ? (g.M - m1 < kPartRows ? g.M - m1 : kPartRows) : 0;
+    float bias[V] = {};
+    if (rows > 0 && !g.part) load_bias<T>(g.epi, n, g.N, true, bias);
 #pragma unroll 2
     for (int r = lane / kLanes; r < rows; r += kRows) {
       float z[V];
@@ -457,7 +476,7 @@ struct TileWork {
       if (g.part)
         store_v(g.part + ((int64_t)split * g.M + m1 + r) * g.N + n, true, V, z);
       else
-        finish<T>(g.epi, m1 + r, n, g.N, z, true);
+        finish<T, STREAM>(g.epi, m1 + r, n, g.N, bias, z, true);
     }
   }
   __device__ __forceinline__ void finish_all(const Gemm &g, const f32x4 (&acc)[FM][FN], char *lds) const {
@@ -475,10 +494,13 @@ struct TileWork {
           *reinterpret_cast<f32x4 *>(turn + (i * 16 + lane % 16) * kPitch + j * 16 + lane / 16 * 4) =
               acc[part * 2 + i][j];
       wave_lds_barrier();
-      if (wide)
-        finish_part<V>(g, m0 + wm + part * kPartRows, turn);
+      const int m1 = m0 + wm + part * kPartRows;
+      if (!wide)
+        finish_part<1, false>(g, m1, turn);
+      else if (g.epi.stream && !g.part)
+        finish_part<V, true>(g, m1, turn);
       else
-        finish_part<1>(g, m0 + wm + part * kPartRows, turn);
+        finish_part<V, false>(g, m1, turn);
       wave_lds_barrier();
     }
   }
@@ -638,7 +660,9 @@ __global__ __launch_bounds__(kBlock) void gemm_join_kernel(const Gemm g) {
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] += v[i];
   }
-  finish<T>(g.epi, m, n, g.N, z, true);
+  float bias[V];
+  load_bias<T>(g.epi, n, g.N, true, bias);
+  finish<T, false>(g.epi, m, n, g.N, bias, z, true);
 }
 
 // ---- few rows ----
@@ -705,7 +729,10 @@ __global__ __launch_bounds__(kRowWaves *kWave) void gemm_rows_kernel(const Gemm 
   for (int s = 1; s < kRowWaves; ++s) sum += red[s][f][lane];
   const int m = f * 16 + i, n = n0 + c * 4;
   float z[4] = {sum.x, sum.y, sum.z, sum.w};
-  if (m < g.M && n < g.N) finish<T>(g.epi, m, n, g.N, z, g.epi.vec);
+  if (m >= g.M || n >= g.N) return;
+  float bias[4];
+  load_bias<T>(g.epi, n, g.N, g.epi.vec, bias);
+  finish<T, false>(g.epi, m, n, g.N, bias, z, g.epi.vec);
 }
 
 // ---- gradient of the activation, and the bias grad's partial sums ----
