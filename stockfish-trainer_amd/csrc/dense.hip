@@ -11,7 +11,6 @@ typedef _Float16 f16_t;
 namespace {
 
 constexpr int kStage = 64;         // bytes of k per pipeline stage
-constexpr int64_t kRowsMost = 64;  // rows the row kernel takes
 constexpr int64_t kCus = 256;
 constexpr int64_t kStrideMost = (int64_t)1 << 23;  // bytes: a tile's rows span less than 32 bits count
 
@@ -29,6 +28,11 @@ int64_t padded(int64_t n, int64_t es) { return (n + 16 / es - 1) & ~(16 / es - 1
 // of the tiles at a time per stage that was measured with many of them (below, us, at
 // 8192^3 and 65536 x 1040 x 4096), each round of workgroups adds its first copies'
 // latency and its results' stores, and partials are written and read at 4 TB/s.
+// Measured both sides of the rule (bf16, us): 8192^3 forward 1550 in 64 x 128 tiles, 1180 in
+// 128 x 128, 816 in 256 x 256; 16384 x 1040 x 1040 input grad 61, 51, 66; 2048^3 weight
+// grad 25, 24, 41; 16384 x 1040 x 128 forward 15, 18, 26 (binary32: input grad 41, 44).
+// Splitting k: weight grad of 16384 x 1040 x 128 108 -> 24 (binary32 549 -> 45), of
+// 65536 x 1040 x 4096 897 -> 520, of 5000 x 1040 x 520 36 -> 22.
 struct Cut {
   int tile, tiles_m, tiles_n, splits, split_k;
 };
@@ -64,6 +68,18 @@ Cut cut_of(int dtype, int64_t M, int64_t N, int64_t K) {
 size_t part_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
   const int s = cut_of(dtype, M, N, K).splits;
   return s > 1 ? a256((size_t)s * M * N * 4) : 0;
+}
+
+// Whether the row kernel takes a forward.  Each of its workgroups reads the rows (in
+// groups of 16, 32 or 64) and 16 outputs' weights itself, which is all it does up to the
+// bytes below; from there on tiles with split k win.  us, row kernel / tiles: bf16 K = 1040,
+// N = 4096 1 row 2.9 / 6.6, 64 rows 5.3 / 10.1; K = 2048, N = 2048 48 rows 9.5 / 9.8, 64 rows
+// 10.9 / 10.2; K = 4096, N = 1040 16 rows 8.9 / 10.9, 32 rows 12.4 / 11.3, 64 rows 19.6 / 12.6;
+// binary32 K = 1040, N = 4096 64 rows 10.7 / 15.2, K = 4096, N = 1040 16 rows 16.0 / 12.5.
+constexpr int64_t kRowsMost = 64, kRowBytesMost = 360 << 10;
+bool few_rows(int64_t M, int64_t K, int64_t es) {
+  const int64_t rows = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  return M <= kRowsMost && (rows + 16) * K * es <= kRowBytesMost;
 }
 
 // A matrix that a product reads: rows of dense elements.
@@ -179,8 +195,8 @@ using namespace dense;
 // Workspace of the forward of these operands; copied: whatever their alignment.
 size_t linear_fwd_workspace(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t M, int64_t K,
                             int64_t N, bool copied) {
-  if (M <= kRowsMost) return 0;
   const int64_t es = type_size(dtype);
+  if (few_rows(M, K, es)) return 0;
   return copy_bytes(Matrix{x, ldx, M, K}, es, copied) + copy_bytes(Matrix{w, ldw, N, K}, es, copied) +
          part_bytes(dtype, M, N, K);
 }
@@ -189,7 +205,7 @@ int linear_fwd(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw
                const void *residual, int64_t ldr, void *y, int64_t ldy, void *deriv, int64_t M, int64_t K, int64_t N,
                int act, void *workspace, hipStream_t s) {
   Epilogue epi{bias, residual, y, act == SFT_ACT_NONE ? nullptr : deriv, ldr, ldy, act, false, false};
-  if (M <= kRowsMost) {
+  if (few_rows(M, K, type_size(dtype))) {
     Gemm g = {};
     g.a = x;
     g.b = w;

@@ -27,11 +27,14 @@ using dense::group_reduce;
 using dense::group_sum;
 
 constexpr int kThreads = 1024;   // of the forward: 16 waves, whose sums leave as one partial
-constexpr int kMaxParts = 512;  // its workgroups, two per CU
+// Its workgroups, one per CU: with two, 524288 x 8 bf16 takes 16.0 us instead of 13.7 and
+// 65536 x 256 31.1 instead of 25.8 (twice the partials to join), 524288 x 64 33 either way.
+constexpr int kMaxParts = 256;
 
 // A row's logits: lane t of the group holds the chunks t + G j of V elements.  Loads
-// have no branches (whole: E is a multiple of V), so that the next row's are under way
-// beside this one's work; open() turns them into numbers, -inf past E.
+// have no branches, so that the next row's are under way beside this one's work; open()
+// turns them into numbers, -inf past E.  WHOLE: E is a multiple of V, and a chunk is one
+// load (524288 x 64 bf16 forward 33 us, element by element 47.5).
 template <typename T, int G, int C, bool WHOLE>
 struct Row {
   static constexpr int V = 16 / (int)sizeof(T);
@@ -232,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restri
   if (gridDim.x > 1) return;
   __threadfence_block();
   __syncthreads();
-  join_parts(part_p, part_c, part_n, 1, E, top_k, loss, counts, kept_rows);  // the only part: no launch for it
+  join_parts(part_p, part_c, part_n, 1, E, top_k, loss, counts, kept_rows);  // the only part: no launch for it (300 x 8 9.4 us, with one 10.7)
 }
 
 __global__ __launch_bounds__(kThreads) void balance_join_kernel(const float *__restrict__ part_p,

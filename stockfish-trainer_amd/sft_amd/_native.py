@@ -845,15 +845,12 @@ def linear_fwd(x, w, bias, residual, y, deriv, act: int) -> None:
     """y = residual + act(x w^T + bias) of 2-D tensors with dense rows; deriv (or None) gets act'."""
     (M, K), N = x.shape, w.shape[0]
     code, dev = type_code(x.dtype), x.device
-    nbytes, keep, ws = 0, None, None
-    if M > 64:  # fewer rows need none
-        n = ctypes.c_size_t(0)
-        _check(lib().sft_linear_fwd_workspace_size(code, M, K, N, _copy_flag(x, w), ctypes.byref(n)),
-               "sft_linear_fwd_workspace_size")
-        nbytes = n.value
-        keep, ws = _scratch(nbytes, dev)
+    n = ctypes.c_size_t(0)
+    _check(lib().sft_linear_fwd_workspace_size(code, M, K, N, _copy_flag(x, w), ctypes.byref(n)),
+           "sft_linear_fwd_workspace_size")
+    keep, ws = _scratch(n.value, dev)
     _call("sft_linear_fwd", dev, code, x.data_ptr(), _rows(x), w.data_ptr(), _rows(w), _at(bias), _at(residual),
-          0 if residual is None else _rows(residual), y.data_ptr(), _rows(y), _at(deriv), M, K, N, act, ws, nbytes)
+          0 if residual is None else _rows(residual), y.data_ptr(), _rows(y), _at(deriv), M, K, N, act, ws, n.value)
     del keep
 
 

@@ -78,6 +78,14 @@ def test_long_sums(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(1, 12000, 50), (16, 5761, 129), (40, 4104, 33), (64, 2049, 24)])
+def test_few_rows_of_long_sums(size, dtype):
+    """Few rows on both sides of the length from which k is split."""
+    announce(f"linear few rows {size} {dtype}")
+    _check(*_inputs(sum(size), *size, dtype), "gelu")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("size", [(50, 64, 40), (300, 128, 136), (150, 72, 33)])
 def test_strides(size, dtype):
     """Slices of wider rows, odd offsets, transposed weights: the values alone count."""
