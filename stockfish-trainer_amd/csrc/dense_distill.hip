@@ -13,8 +13,10 @@
 // waves that hold it, as loaded, until the gradient; rows longer than a workgroup's
 // registers are read again, from L2 or the memory-side cache.  Rows start anywhere, so
 // they are cut at the logits' 16-byte lines: whole chunks, and the few elements before
-// and after them one a thread.  All loads of a row
-// are made without branches, so that they are under way together.
+// and after them one a thread.  All loads of a row are made without branches, so that
+// they are under way together.  Long rows hold a CU with one workgroup whose reading,
+// reducing and writing follow each other: 2048 x 100003 bf16 takes 97 us for the loss and
+// 218 for the gradient, 4.2 and 3.8 TB/s.
 #include "dense.h"
 #include "dense_reduce.h"
 
@@ -295,6 +297,13 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
       ds[te.idx[j]] = (T)(gp * __builtin_amdgcn_exp2f(((float)s[te.idx[j]] - m) * c2) - g * total[j]);
 }
 
+// A row goes to the fewest waves whose registers hold it: a row of one wave needs no
+// meeting, and no chunk slot should be idle.  us of loss and gradient in bf16, k = 32, as
+// chosen / with the next larger form of the list: 65536 x 512 104 / 154 and 32768 x 2048
+// 81 / 90 (a wave / a workgroup), 16384 x 4096 65 / 82 (8 chunks of a wave / 4 of four waves),
+// 8192 x 16384 115 / 149, 2048 x 49152 84 / 98 (6 chunks / 8), 2048 x 104000 187 / 210 (13 / 16).
+// Rows beyond 16 chunks of 16 waves are read twice: 1024 x 131000 143 held, 150 read twice.
+// At 16384 x 4096 the rows are read and written at 4.3 TB/s, what a copy reaches.
 template <typename T>
 void launch(const Distill &d, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
