@@ -11,6 +11,8 @@ enum Layout { kForward = 0, kInputGrad = 1, kWeightGrad = 2 };
 // Tiles of a product: 64 x 128, 128 x 128 and, of 16-bit types, 256 x 256.
 enum TileKind { kTile64 = 0, kTile128 = 1, kTile256 = 2 };
 
+constexpr int kWaveCols = 64;  // columns of a tile's waves
+
 // What becomes of a product's sums: y = residual + act(sum + bias), rounded once.
 struct Epilogue {
   const void *bias;      // [N] or null
@@ -33,6 +35,7 @@ struct Gemm {
   int tile, tiles_m, tiles_n;
   int splits, split_k;  // k per split, whole stages
   float *part;          // [splits][M][N] when splits > 1
+  float *sums;          // [splits][M] sums of A over k, or null: of weight grads with a spare wave
   Epilogue epi;
 };
 
@@ -55,7 +58,9 @@ int launch_gemm(const Gemm &g, int layout, hipStream_t s);
 template <typename T>
 int launch_rows(const Gemm &g, hipStream_t s);
 template <typename T>
-int launch_act_bwd(const ActBwd &p, void *db, hipStream_t s);
+int launch_act_bwd(const ActBwd &p, hipStream_t s);
+template <typename T>
+int launch_bias_join(const float *part, int parts, int N, void *db, hipStream_t s);
 template <typename T>
 int launch_align(const Copy &a, const Copy &b, hipStream_t s);
 

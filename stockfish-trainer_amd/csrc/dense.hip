@@ -129,7 +129,7 @@ bool epilogue_vec(const Epilogue &e, int64_t N, int64_t es, int64_t V) {
 
 // C [M, N] of operands that are read in place.
 int run_gemm(int dtype, int layout, const Matrix &a, const Matrix &b, int64_t M, int64_t N, int64_t K,
-             const Epilogue &epi, Scratch ws, hipStream_t s) {
+             const Epilogue &epi, float *sums, Scratch ws, hipStream_t s) {
   const int64_t es = type_size(dtype);
   const bool ak = layout != kWeightGrad, bk = layout == kForward;
   Gemm g = {};
@@ -158,9 +158,20 @@ int run_gemm(int dtype, int layout, const Matrix &a, const Matrix &b, int64_t M,
   g.tiles_n = c.tiles_n;
   g.splits = c.splits;
   g.split_k = c.split_k;
+  g.sums = sums;
   g.part = c.splits > 1 ? static_cast<float *>(ws.take(0)) : nullptr;
   ProfScope prof(kProfDenseProduct, s);
   return SFT_DENSE_CALL(dtype, launch_gemm, g, layout, s);
+}
+
+// The bias grad without an activation, from the weight grad's product: where its last tiles
+// have a wave past the last column, that wave sums dy instead of idling, and dy is not read
+// for it: 65536 x 1040 x 4096 bf16 1.81 -> 1.71 ms a step.  Else, and of binary32, whose products take
+// six instructions, dy is read once more.  Returns the number of partials, 0 for else.
+int product_sums(int dtype, bool dw, int64_t M, int64_t K, int64_t N, int act) {
+  if (!dw || act != SFT_ACT_NONE || dtype == SFT_TYPE_F32) return 0;
+  const Cut c = cut_of(dtype, N, K, M);
+  return ceil_div(K, kWaveCols) * kWaveCols < (int64_t)c.tiles_n * kTiles[c.tile].cols ? c.splits : 0;
 }
 
 // The shape of the activation's backward and bias sums: about 1024 workgroups.
@@ -222,7 +233,7 @@ int linear_fwd(int dtype, const void *x, int64_t ldx, const void *w, int64_t ldw
   Scratch ws{static_cast<char *>(workspace)};
   Matrix a{x, ldx, M, K}, b{w, ldw, N, K};
   const int rc = align(dtype, &a, &b, ws, s);
-  return rc ? rc : run_gemm(dtype, kForward, a, b, M, N, K, epi, ws, s);
+  return rc ? rc : run_gemm(dtype, kForward, a, b, M, N, K, epi, nullptr, ws, s);
 }
 
 size_t linear_bwd_workspace(int dtype, const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w,
@@ -234,7 +245,8 @@ size_t linear_bwd_workspace(int dtype, const void *dy, int64_t lddy, const void 
   shape_act_bwd(dtype, M, N, p);
   const Matrix g{dy, lddy, M, N};
   size_t n = act != SFT_ACT_NONE ? g.copy_bytes(es) : dx || dw ? copy_bytes(g, es, copied) : 0;
-  if (db) n += a256((size_t)p.parts * N * 4);
+  const int sums = product_sums(dtype, dw, M, K, N, act);
+  if (db) n += a256((size_t)(sums ? sums : p.parts) * N * 4);
   if (dx) n += copy_bytes(Matrix{w, ldw, N, K}, es, copied);
   if (dw) n += copy_bytes(Matrix{x, ldx, M, K}, es, copied);
   const size_t in = dx ? part_bytes(dtype, M, K, N) : 0, weight = dw ? part_bytes(dtype, N, K, M) : 0;
@@ -262,21 +274,27 @@ int linear_bwd(int dtype, const void *dy, int64_t lddy, const void *deriv, const
     p.dz = ws.take(dz.copy_bytes(es));
     dz = Matrix{p.dz, p.lddz, M, p.lddz};
   }
-  if (db) p.part = static_cast<float *>(ws.take(a256((size_t)p.parts * N * 4)));
+  const int sums = product_sums(dtype, dw, M, K, N, act), parts = sums ? sums : p.parts;
+  if (db) p.part = static_cast<float *>(ws.take(a256((size_t)parts * N * 4)));
   int rc = SFT_OK;
-  if (db || act != SFT_ACT_NONE) {
+  if (act != SFT_ACT_NONE || (db && !sums)) {
     ProfScope prof(kProfDenseActBwd, s);
-    rc = SFT_DENSE_CALL(dtype, launch_act_bwd, p, db, s);
+    rc = SFT_DENSE_CALL(dtype, launch_act_bwd, p, s);
   }
   Matrix in{x, ldx, M, K}, weight{w, ldw, N, K};
   if (!rc && (dx || dw)) rc = align(dtype, &dz, nullptr, ws, s);
   if (!rc) rc = align(dtype, dx ? &weight : nullptr, dw ? &in : nullptr, ws, s);
   if (!rc && dx)
     rc = run_gemm(dtype, kInputGrad, dz, weight, M, K, N,
-                  Epilogue{nullptr, nullptr, dx, nullptr, 0, K, SFT_ACT_NONE, false, false}, ws, s);
+                  Epilogue{nullptr, nullptr, dx, nullptr, 0, K, SFT_ACT_NONE, false, false}, nullptr, ws, s);
   if (!rc && dw)
     rc = run_gemm(dtype, kWeightGrad, dz, in, N, K, M,
-                  Epilogue{nullptr, nullptr, dw, nullptr, 0, K, SFT_ACT_NONE, false, false}, ws, s);
+                  Epilogue{nullptr, nullptr, dw, nullptr, 0, K, SFT_ACT_NONE, false, false}, sums ? p.part : nullptr,
+                  ws, s);
+  if (!rc && db) {
+    ProfScope prof(kProfDenseActBwd, s);
+    rc = SFT_DENSE_CALL(dtype, launch_bias_join, p.part, parts, (int)N, db, s);
+  }
   return rc;
 }
 

@@ -593,6 +593,7 @@ __global__ __launch_bounds__(WM *WN *kWave, BM / WM * BN / WN > 128 * 64 ? 1 : 2
     clip();
     copy(ring_to + s * kStage);
   }
+  static_assert(BN / WN == kWaveCols, "the rule for spare waves");
   Frag<T> fa[2][FM], fb[2][FN];
   meet(std::integral_constant<int, RING - MEET>{});  // stage 0
   read(ring, fa[0], fb[0]);
@@ -630,6 +631,37 @@ __global__ __launch_bounds__(WM *WN *kWave, BM / WM * BN / WN > 128 * 64 ? 1 : 2
           at = next(at);
           slot = next(slot);
         }
+      }
+    }
+  } else if (!AK && !kPairs && g.sums && w.m0 + w.wm < g.M && w.n0 + w.wn - g.N < kWaveCols) {
+    // The first wave past the last column: the sums of A over k, as products with ones.
+    Frag<T> ones;
+    ones.v = u32x4{1u, 1u, 1u, 1u} * (std::is_same<T, bf16_t>::value ? 0x3f803f80u : 0x3c003c00u);
+    auto copy_read_a = [&](SFT_LDS char *__restrict__ to, const SFT_LDS char *__restrict__ from, Frag<T>(&f)[FM]) {
+      la.load(to);
+      lb.load(to + BM * kStageBytes);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) f[i] = ra.read(from, i);
+    };
+    for (int s = 0; s < steps; s += 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (s + h < steps) {
+          clip();
+          if (h % MEET == 0) meet(Under{});
+          copy_read_a(ring_to + at * kStage, ring + slot * kStage, fa[1 - h]);
+#pragma unroll
+          for (int i = 0; i < FM; ++i) acc[i][0] = Mma<T>::step(ones, fa[h][i], acc[i][0], 0);
+          at = next(at);
+          slot = next(slot);
+        }
+      }
+    }
+    if (lane_id() < 16) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int m = w.m0 + w.wm + i * 16 + lane_id();
+        if (m < g.M) g.sums[(int64_t)w.split * g.M + m] = acc[i][0].x;
       }
     }
   } else {  // a wave past the edge: its share of the copies only
@@ -871,14 +903,18 @@ int launch_rows(const Gemm &g, hipStream_t s) {
 }
 
 template <typename T>
-int launch_act_bwd(const ActBwd &p, void *db, hipStream_t s) {
+int launch_act_bwd(const ActBwd &p, hipStream_t s) {
   const int64_t chunks = ceil_div(p.N, 16 / (int64_t)sizeof(T));
   hipLaunchKernelGGL((act_bwd_kernel<T>), dim3((unsigned)ceil_div(chunks, p.tx), (unsigned)p.parts), dim3(kBlock), 0, s,
                      p);
-  if (db)
-    hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)ceil_div(p.N, kJoinCols)), dim3(kJoinCols * kJoinRows), 0,
-                       s, p.part, p.parts, p.N, db);
   return check_launch("dense activation backward");
+}
+
+template <typename T>
+int launch_bias_join(const float *part, int parts, int N, void *db, hipStream_t s) {
+  hipLaunchKernelGGL((bias_join_kernel<T>), dim3((unsigned)ceil_div(N, kJoinCols)), dim3(kJoinCols * kJoinRows), 0, s,
+                     part, parts, N, db);
+  return check_launch("dense bias grad");
 }
 
 template <typename T>
@@ -892,7 +928,8 @@ int launch_align(const Copy &a, const Copy &b, hipStream_t s) {
 #define SFT_DENSE_TYPE(T)                                                \
   template int launch_gemm<T>(const Gemm &, int, hipStream_t);           \
   template int launch_rows<T>(const Gemm &, hipStream_t);                \
-  template int launch_act_bwd<T>(const ActBwd &, void *, hipStream_t);   \
+  template int launch_act_bwd<T>(const ActBwd &, hipStream_t);           \
+  template int launch_bias_join<T>(const float *, int, int, void *, hipStream_t); \
   template int launch_align<T>(const Copy &, const Copy &, hipStream_t);
 
 }  // namespace dense

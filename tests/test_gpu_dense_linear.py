@@ -86,6 +86,34 @@ def test_few_rows_of_long_sums(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [(1, 8, 5), (70, 64, 300), (300, 136, 130), (700, 100, 129), (500, 1040, 264),
+                                  (9000, 72, 40), (6000, 1040, 2050)])
+def test_bias_grads_without_an_activation(size, dtype):
+    """K with and without spare columns in the weight grad's last tiles, one part and many."""
+    announce(f"linear bias grad {size} {dtype}")
+    _check(*_inputs(sum(size), *size, dtype, residual=False), "none")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_bias_grad_alone(dtype):
+    """Without the weight grad, and with non-finite gradients in one column."""
+    announce(f"linear bias grad alone {dtype}")
+    x, w, b, _, dy = _inputs(1, 200, 72, 40, dtype)
+    dy[3, 7], dy[5, 9] = float("inf"), float("nan")
+    xd, wd, bd = (t.to(DEV) for t in (x, w, b))
+    bd.requires_grad_()
+    alone, = torch.autograd.grad(fused_linear(xd, wd, bd), bd, dy.to(DEV))
+    wd.requires_grad_()
+    _, both = torch.autograd.grad(fused_linear(xd, wd, bd), (wd, bd), dy.to(DEV))
+    value = dy.double().sum(0)
+    bound = dense_ref.rounded((200 + 3) * dense_ref.U32 * dy.double().abs().sum(0), value, dtype)
+    for got in (alone.cpu().double(), both.cpu().double()):
+        assert torch.isinf(got[7]) and torch.isnan(got[9])
+        rest = torch.isfinite(value)
+        assert ((got - value).abs() <= bound)[rest].all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("size", [(50, 64, 40), (300, 128, 136), (150, 72, 33)])
 def test_strides(size, dtype):
     """Slices of wider rows, odd offsets, transposed weights: the values alone count."""
