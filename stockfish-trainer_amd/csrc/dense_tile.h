@@ -337,6 +337,9 @@ __device__ __forceinline__ void mma_all(const Frag<T> (&fa)[FM], const Frag<T> (
 // 2^-24 of the whole are added, in binary32.  What is left out and the sums' own
 // rounding are of the size of a binary32 product's rounding; a row with an infinity
 // becomes NaN (inf - inf) where a binary32 product would keep the infinity.
+// 65536 x 1040 x 128 forward 98 us, 178 TFLOP/s, where the binary32 instructions' products
+// of 8192^3 come to 153.  Bound by the vector work of the splitting, about as long as the
+// products beside it.
 // One fragment of each part: 8 k of a lane, 4 from each of two stages.
 struct Split {
   u32x4 part[3];
@@ -512,6 +515,13 @@ struct TileWork {
 // the past ones are free, and as many copies are made.  The copies carry their own
 // bounds checks, so those past the end are made too (they give zeros) and every
 // meeting waits for the same number of outstanding ones.
+//
+// Bound by feeding the matrix cores: with 256 x 256 tiles, which read least from LDS and
+// memory a product, 8192^3 bf16 runs at 1.35 to 1.41 PFLOP/s; the cores are busy 65% of the
+// cycles, LDS has no bank conflicts, and waves spend 30% of their time at the meetings.
+// 65536 x 1040 x 4096, us: forward 573 (0.97 PFLOP/s; its 537 MB of results take 115 at a
+// copy's rate), input grad 524, weight grad 520.  Smaller tiles have several workgroups a
+// CU, one's copies and results under another's products: 16384 x 1040 x 1040 59, 51, 54.
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int RING, int MEET>
 __global__ __launch_bounds__(WM *WN *kWave, BM / WM * BN / WN > 128 * 64 ? 1 : 2) void gemm_ring_kernel(const Gemm g) {
   typedef TileWork<T, BM, BN, WM, WN> Work;
@@ -675,7 +685,9 @@ __global__ __launch_bounds__(WM *WN *kWave, BM / WM * BN / WN > 128 * 64 ? 1 : 2
   w.finish_all(g, acc, lds);
 }
 
-// Sums a split product's partials in split order and finishes them; V elements a thread.
+// Sums a split product's partials in split order and finishes them; V elements a thread,
+// with the loads of 8 splits under way.  Bound by those, from the memory-side cache: 6.5 us
+// for the weight grad of 16384 x 1040 x 1040.
 template <typename T, int V>
 __global__ __launch_bounds__(kBlock) void gemm_join_kernel(const Gemm g) {
   const int64_t vecs = g.N / V;  // N is a multiple of V
@@ -700,7 +712,8 @@ __global__ __launch_bounds__(kBlock) void gemm_join_kernel(const Gemm g) {
 // ---- few rows ----
 // y for up to 16 FM rows: a workgroup holds 16 outputs of every row; its waves take
 // 256-byte pieces of k in turn, straight from global memory (W is read once and
-// there is no reuse for LDS to serve), and are summed in wave order.
+// there is no reuse for LDS to serve), and are summed in wave order.  Bound by the latency
+// of W's one read, then by its rate: a row x 1040 x 4096 bf16 2.9 us (2.9 TB/s), 64 rows 5.3.
 constexpr int kRowWaves = 8;
 template <typename T, int FM>
 __global__ __launch_bounds__(kRowWaves *kWave) void gemm_rows_kernel(const Gemm g) {
@@ -771,8 +784,8 @@ __global__ __launch_bounds__(kRowWaves *kWave) void gemm_rows_kernel(const Gemm 
 // dz = dy * act'(z), rounded to the layer's type for the products that follow (its
 // rows are padded with zeros to whole chunks), and the sums of the unrounded dz over
 // `rows` rows per workgroup and column.  A thread holds a chunk of V columns; a
-// workgroup is tx chunks by 256 / tx rows.  Reading and writing bound it: 4.6 TB/s at
-// 65536 x 4096.
+// workgroup is tx chunks by 256 / tx rows.  Reading and writing bound it: 16384 x 1040 bf16
+// 20 us, 5.1 TB/s, the sums alone at 65536 x 4096 4.8 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
   typedef typename Deriv<T>::type D;
@@ -822,7 +835,7 @@ __global__ __launch_bounds__(kBlock) void act_bwd_kernel(const ActBwd p) {
 }
 
 // db[n] = the sum of column n's partials: 64 threads take every 64th each, and are
-// added in order.
+// added in order.  4 us, mostly the launch and one round of loads.
 constexpr int kJoinCols = 16, kJoinRows = 64;
 template <typename T>
 __global__ __launch_bounds__(kJoinCols *kJoinRows) void bias_join_kernel(const float *__restrict__ part, int parts,
@@ -844,7 +857,9 @@ __global__ __launch_bounds__(kJoinCols *kJoinRows) void bias_join_kernel(const f
 
 // ---- copies of operands with whole, aligned rows ----
 // Up to two matrices of rows x cols elements, to rows of a whole number of chunks with
-// zeros past cols.  One chunk a thread.
+// zeros past cols.  One chunk a thread: 5003 x 1037 f16 5.6 us, 3.7 TB/s.  (Operands read in
+// place by guarded loads through registers, in the product itself, were slower: every
+// tile pays for them again.)
 template <typename T>
 __global__ __launch_bounds__(kBlock) void align_rows_kernel(const Copy a, const Copy b, int64_t blocks_a) {
   const bool second = (int64_t)blockIdx.x >= blocks_a;
@@ -860,6 +875,9 @@ __global__ __launch_bounds__(kBlock) void align_rows_kernel(const Copy a, const 
 template <typename T, bool AK, bool BK>
 int launch_gemm_as(const Gemm &g, hipStream_t s) {
   const int64_t grid = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  // Rings as deep as keep three workgroups of the smaller tiles on a CU (48 KB each) and one
+  // of the largest (128 of 160 KB; 5 slots: the same 1.24 PFLOP/s of 8192^3 at that time; a
+  // meeting in two stages 1.16).
 #define SFT_RING(BM, BN, WM, WN, RING, MEET)                                                                  \
   hipLaunchKernelGGL((gemm_ring_kernel<T, AK, BK, BM, BN, WM, WN, RING, MEET>), dim3((unsigned)grid),         \
                      dim3(WM *WN *kWave), 0, s, g)
