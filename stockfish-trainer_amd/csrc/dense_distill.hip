@@ -73,20 +73,21 @@ __device__ __forceinline__ float load_type(const void *p, int64_t i, int type) {
 
 // The teacher's side of a row, in one wave: lane l holds the slots l + 64 j.
 struct Teacher {
-  int idx[kSlots];    // class, or -1
-  float q[kSlots];    // probability
-  float cross;        // sum_j q_j (log q_j - s_{i_j} / tau)
+  int idx[kSlots];     // class, or -1
+  float q[kSlots];     // probability
+  float log_q[kSlots];
+  float at[kSlots];    // the student's logit there
   bool any;
   template <typename T>
   __device__ __forceinline__ void load(const Distill &d, int64_t row, const T *s) {
     const int lane = lane_id();
     const float c = 1.f / d.tau;
-    float t[kSlots], at[kSlots], m = -INFINITY;
+    float t[kSlots], m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       idx[j] = -1;
       t[j] = -INFINITY;
-      at[j] = 0.f;
+      log_q[j] = at[j] = 0.f;
       if (j * kWave >= d.k) continue;  // uniform
       const int slot = lane + j * kWave;
       if (slot < d.k) {
@@ -94,8 +95,8 @@ struct Teacher {
         const int64_t i = d.idx64 ? static_cast<const int64_t *>(d.idx)[o] : static_cast<const int32_t *>(d.idx)[o];
         if (i >= 0 && i < d.V) {
           idx[j] = (int)i;
-          t[j] = load_type(d.t, o, d.ttype) * c;
-          at[j] = (float)s[i] * c;
+          t[j] = load_type(d.t, o, d.ttype);
+          at[j] = (float)s[i];
         }
       }
       m = t[j] > m || t[j] != t[j] ? t[j] : m;  // a NaN stays
@@ -107,19 +108,30 @@ struct Teacher {
     for (int j = 0; j < kSlots; ++j) {
       q[j] = 0.f;
       if (j * kWave >= d.k) continue;
-      q[j] = any ? expf(t[j] - m) : 0.f;
+      log_q[j] = any ? (t[j] - m) * c : 0.f;
+      q[j] = any ? expf(log_q[j]) : 0.f;
       sum += q[j];
     }
     sum = dense::group_sum<kWave>(sum);
     const float inv = any ? 1.f / sum : 0.f, log_sum = any ? logf(sum) : 0.f;
-    cross = 0.f;
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       if (j * kWave >= d.k) continue;
       q[j] *= inv;
-      if (q[j] != 0.f) cross += q[j] * (t[j] - m - log_sum - at[j]);
+      log_q[j] -= log_sum;
     }
-    cross = dense::group_sum<kWave>(cross);
+  }
+  // sum_j q_j (log q_j - log p_{i_j}), of a student's row with maximum m and sum of
+  // exponentials: taken slot by slot, since sums of either part would cancel.
+  __device__ __forceinline__ float divergence(const Distill &d, float m, float sum) const {
+    const float c = 1.f / d.tau, log_sum = logf(sum);
+    float all = 0.f;
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      if (j * kWave >= d.k) continue;
+      if (q[j] != 0.f) all += q[j] * (log_q[j] - ((at[j] - m) * c - log_sum));
+    }
+    return dense::group_sum<kWave>(all);
   }
   // q of the class of slot j, over all its slots (classes may be named twice).
   __device__ __forceinline__ void merged(int k, float (&total)[kSlots]) const {
@@ -162,10 +174,11 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
   constexpr int V = 16 / (int)sizeof(T), kWaves = TPR / kWave;
   constexpr int kRowsPer = TPR == kWave ? kWavesPerBlock : 1;
   __shared__ float top[kWaves], sums[kWaves];
-  __shared__ float shared_cross;
   __shared__ int shared_any;
   __shared__ int slot_idx[kWaves > 1 ? SFT_DISTILL_MAX_K : 1];  // the teacher's side, until the end
   __shared__ float slot_q[kWaves > 1 ? SFT_DISTILL_MAX_K : 1];
+  __shared__ float slot_log_q[kWaves > 1 ? SFT_DISTILL_MAX_K : 1];
+  __shared__ float slot_at[kWaves > 1 ? SFT_DISTILL_MAX_K : 1];
   const int tid = threadIdx.x % TPR, wave = uniform(tid / kWave);
   const int64_t row = (int64_t)blockIdx.x * kRowsPer + uniform(threadIdx.x / TPR);
   if (row >= d.rows) return;  // whole waves, and never part of a row's
@@ -204,6 +217,8 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
       for (int j = 0; j < kSlots; ++j) {
         slot_idx[lane_id() + j * kWave] = te.idx[j];
         slot_q[lane_id() + j * kWave] = te.q[j];
+        slot_log_q[lane_id() + j * kWave] = te.log_q[j];
+        slot_at[lane_id() + j * kWave] = te.at[j];
       }
     }
   }
@@ -236,22 +251,33 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
       top[wave] = run.m;
       sums[wave] = run.sum;
     }
-    if (tid == 0) {
-      shared_cross = te.cross;
-      shared_any = te.any;
-    }
+    if (tid == 0) shared_any = te.any;
     __syncthreads();
     // every wave joins the waves' results, in the same order
     const int l = lane_id();
     run.m = l < kWaves ? top[l] : -INFINITY;
     run.sum = l < kWaves ? sums[l] : 0.f;
     run.join(c2);
-    te.cross = shared_cross;
     te.any = shared_any;
   }
   const float m = run.m, sum = run.sum;
   const bool live = te.any && m > -INFINITY;
-  if (d.loss && tid == 0) d.loss[row] = live ? d.tau * d.tau * (te.cross + m / d.tau + logf(sum)) : 0.f;
+  auto put_loss = [&]() {
+    if (!d.loss || wave != 0) return;
+    if (kWaves > 1) {
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) {
+        te.q[j] = slot_q[lane_id() + j * kWave];
+        te.log_q[j] = slot_log_q[lane_id() + j * kWave];
+        te.at[j] = slot_at[lane_id() + j * kWave];
+      }
+    }
+    const float kl = te.divergence(d, m, sum);
+    if (tid == 0) d.loss[row] = live ? d.tau * d.tau * kl : 0.f;
+  };
+  // With a gradient to come, a workgroup's loss waits until the row has left the registers:
+  // beside it 2048 x 49152 bf16 takes 95 us instead of 84.
+  if (kWaves == 1 || !d.ds) put_loss();
   if (!d.ds) return;
 
   const float g = d.tau * (d.weight ? d.weight[row] : 1.f), gp = g / sum;
@@ -277,6 +303,7 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
     }
   }
   if (tid < edge) ds[mine] = (T)grad(x_edge);
+  if (kWaves > 1) put_loss();
   if (!live) return;  // the same for the whole row
   // The teacher's classes once more, after the stores above have been made.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

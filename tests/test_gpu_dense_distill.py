@@ -88,6 +88,20 @@ def test_a_class_the_student_excludes_costs_infinitely_much():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,k", [(146, 146), (5000, 256), (40000, 200)])
+def test_logits_far_from_zero_and_teachers_that_agree(V, k, dtype):
+    """The loss is a difference of logits: neither their common offset nor log-sums may show in its error."""
+    announce(f"distill offset {V} {k} {dtype}")
+    g = torch.Generator().manual_seed(V)
+    s = (1000 + 2 * torch.randn(6, V, generator=g)).to(dtype)
+    i = torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(6)])
+    t = s.float().gather(1, i) + 0.01 * torch.randn(6, k, generator=g)
+    (loss_ref, _) = dense_ref.distill(s.float() - 1000, t - 1000, i, 2.0)  # exact differences
+    loss, _ = distill_loss_and_grad(s.to(DEV), t.to(DEV), i.to(DEV), None, 2.0)
+    assert dense_ref.worst(loss, loss_ref) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_classes_named_twice(dtype):
     announce(f"distill repeated {dtype}")
     s, t, i, w = _inputs(4, 6, 90, 70, dtype, empty=False)
