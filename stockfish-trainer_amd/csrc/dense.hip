@@ -246,7 +246,8 @@ size_t linear_bwd_workspace(int dtype, const void *dy, int64_t lddy, const void 
   const Matrix g{dy, lddy, M, N};
   size_t n = act != SFT_ACT_NONE ? g.copy_bytes(es) : dx || dw ? copy_bytes(g, es, copied) : 0;
   const int sums = product_sums(dtype, dw, M, K, N, act);
-  if (db) n += a256((size_t)(sums ? sums : p.parts) * N * 4);
+  // the size for all grads covers calls for some: without dw the bias's partials are p.parts
+  if (db) n += a256((size_t)(sums > p.parts ? sums : p.parts) * N * 4);
   if (dx) n += copy_bytes(Matrix{w, ldw, N, K}, es, copied);
   if (dw) n += copy_bytes(Matrix{x, ldx, M, K}, es, copied);
   const size_t in = dx ? part_bytes(dtype, M, K, N) : 0, weight = dw ? part_bytes(dtype, N, K, M) : 0;

@@ -88,6 +88,23 @@ def test_linear_bwd_refuses(at, value, needle):
     assert rc == -1 and needle in why
 
 
+@pytest.mark.parametrize("act", [0, 5])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("M,K,N", [(128, 1040, 1040), (1000, 1040, 520), (70, 24, 16), (20000, 136, 264)])
+def test_linear_bwd_workspace_covers_any_grads(M, K, N, dtype, act):
+    """The size is asked for before it is known which grads a step needs."""
+    n = ctypes.c_size_t(0)
+    assert _native.lib().sft_linear_bwd_workspace_size(dtype, M, K, N, act, 0, ctypes.byref(n)) == 0
+    for grads in range(1, 8):
+        dx, dw, db = (P if grads & bit else None for bit in (1, 2, 4))
+        args = [dtype, P, N, P, P, K, P, K, dx, dw, db, M, K, N, act, ctypes.c_void_p(0x1010), 1 << 50, None]
+        if act == 0 and not db:
+            continue  # may need none, and then the call would not be refused
+        rc, why = _call("sft_linear_bwd", args)  # refused: the workspace is not aligned
+        assert rc == _native.SFT_EWORKSPACE
+        assert int(re.search(r"needs (\d+) bytes", why).group(1)) <= n.value, grads
+
+
 # dtype, logits, ld, mask, rows, experts, top_k, loss, counts, kept, ws, ws_bytes, stream
 BALANCE = [0, P, 8, None, 10, 8, 1, P, P, P, None, 0, None]
 

@@ -195,6 +195,19 @@ def test_only_the_grads_asked_for():
             assert dense_ref.worst(v, ref[n]) <= 1.0, n
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_bias_beside_a_frozen_weight(dtype):
+    announce(f"linear frozen weight {dtype}")
+    x, w, b, _, dy = _inputs(6, 128, 1040, 1040, dtype, residual=False)
+    ref = dense_ref.linear(x, w, b, None, "none", dy)
+    for need_x in (False, True):
+        xd, bd = x.to(DEV).requires_grad_(need_x), b.to(DEV).requires_grad_()
+        y = fused_linear(xd, w.to(DEV), bd)
+        got = torch.autograd.grad(y, [bd, xd][:1 + need_x], dy.to(DEV))
+        for n, v in zip(("db", "dx"), got):
+            assert dense_ref.worst(v, ref[n]) <= 1.0, n
+
+
 def test_grads_against_differences():
     """Central differences of the 32-bit forward along random directions: with step h the
     difference quotient is off by h^2 |f'''| / 6 and by the forward's rounding over h."""
