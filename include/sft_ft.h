@@ -535,7 +535,7 @@ int sft_balance_bwd(int32_t dtype, const void *logits, int64_t ld, const uint8_t
  *   loss[row] = T^2 sum_j q_j (log q_j - log p_{i_j})
  *   grad_student[row] = row_weight[row] (1 if NULL) T (p - q): dense [rows, classes]
  * Either output may be NULL.  Slots with q = 0 add nothing.  A row without a filled
- * slot above -inf, or without a class above -inf, has loss 0 and gradient 0.
+ * slot above -inf, or with all classes at -inf, has loss 0 and gradient 0.
  * row_weight and loss are float.
  */
 #define SFT_DISTILL_MAX_K 256

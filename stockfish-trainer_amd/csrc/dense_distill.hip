@@ -5,8 +5,8 @@
 //   loss = tau^2 sum_j q_j (log q_j - log p_{i_j})
 //   d loss / d s_v = tau (p_v - sum of q_j over the slots of class v)
 // Slots with q = 0 add nothing, whatever the student says there.  A row without a
-// filled slot (or whose teacher logits are all -inf), or without a class above -inf,
-// has loss 0 and no gradient.
+// filled slot (or whose teacher logits are all -inf), or with all classes at -inf, has
+// loss 0 and no gradient; a NaN anywhere in a taught row makes both NaN.
 //
 // Bound by reading the logits once and writing the gradient once.  A row is read as it
 // comes, with a running maximum and sum per thread, and stays in the registers of the
@@ -261,7 +261,8 @@ __global__ __launch_bounds__(TPR == kWave ? kBlock : TPR) void distill_kernel(co
     te.any = shared_any;
   }
   const float m = run.m, sum = run.sum;
-  const bool live = te.any && m > -INFINITY;
+  // a row whose numbers are all NaN or -inf has no maximum either, but its sum is NaN
+  const bool live = te.any && (m > -INFINITY || sum != 0.f);
   auto put_loss = [&]() {
     if (!d.loss || wave != 0) return;
     if (kWaves > 1) {

@@ -10,7 +10,8 @@ softmax(teacher / T) over the row's filled slots,
 Slots with an index outside [0, V) are empty, and a class may be named twice.  Classes
 the student excludes hold -inf: they get no probability and no gradient, unless the
 teacher names one with q > 0 (the loss is then infinite).  A row without a
-filled slot, or whose classes are all excluded, has loss 0 and no gradient.
+filled slot, or whose classes are all excluded, has loss 0 and no gradient; a NaN
+in any other row makes its loss and gradient NaN.
 
 distill_loss is differentiable in the student's logits and reads them once more
 in its backward; distill_loss_and_grad makes both in one pass, for loops that

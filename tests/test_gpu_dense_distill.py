@@ -112,6 +112,21 @@ def test_classes_named_twice(dtype):
     _check(s, t, i, w, 0.7)
 
 
+@pytest.mark.parametrize("V", [5, 300, 5000, 20011])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_nan_are_not_taken_for_excluded_ones(V, dtype):
+    announce(f"distill rows of NaN V={V} {dtype}")
+    s, t, i, w = _inputs(5, 70, V, 4, dtype)
+    i[1:] = i[1:].clamp(min=0)  # taught
+    s[3], s[4], s[5] = float("nan"), -float("inf"), -float("inf")
+    s[5, V - 1] = float("nan")
+    loss, ds = distill_loss_and_grad(s.to(DEV), t.to(DEV), i.to(DEV), w.to(DEV))
+    assert torch.isnan(loss[[3, 5]]).all() and torch.isnan(ds[[3, 5]]).all()
+    assert loss[4].item() == 0.0 and torch.equal(ds[4], torch.zeros_like(ds[4]))
+    kept = [r for r in range(70) if r not in (3, 5)]
+    assert not torch.isnan(loss[kept]).any() and not torch.isnan(ds[kept]).any()
+
+
 def test_nan_stays_in_its_row():
     announce("distill NaN")
     s, t, i, w = _inputs(5, 70, 300, 5, torch.bfloat16)
