@@ -509,7 +509,7 @@ int sft_linear_bwd(int32_t dtype, const void *dy, int64_t lddy, const void *deri
  *   p = softmax(logits) per position; its top_k experts are chosen by logit, equal
  *   ones by the lower number, never one at -inf
  *   counts[e] = positions that chose e; *kept = n, the positions that count: not
- *   masked, and with a logit above -inf
+ *   masked, and not all at -inf
  *   *loss = experts * sum_e (counts[e] / (n top_k)) (sum of p_e / n); 0 if n = 0
  * The backward writes dense grad_logits [rows, experts] = *grad_loss times the
  * loss's gradient, the counts held constant; zeros for positions left out, whatever

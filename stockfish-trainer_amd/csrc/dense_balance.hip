@@ -3,8 +3,8 @@
 //   counts_e = #{t : e in S_t},  f_e = counts_e / (n top_k),  P_e = mean_t p_te
 //   loss     = E sum_e f_e P_e
 //   d loss / d logit_tj = E / n p_tj (f_j - sum_e f_e p_te)      (f is piecewise constant)
-// A position is kept if its mask byte is set (or there is no mask) and some logit is
-// above -inf.  Experts are chosen by logit, equal ones by the lower number; those at
+// A position is kept if its mask byte is set (or there is no mask) and not all its logits
+// are -inf; a NaN in a kept one makes the loss NaN.  Experts are chosen by logit, equal ones by the lower number; those at
 // -inf are never chosen.
 //
 // Bound by reading the logits (and, in the backward, writing as much): every row is
@@ -68,8 +68,10 @@ struct Row {
       for (int i = 0; i < V; ++i) m = fmaxf(m, x[j][i]);
     return group_max<G>(m);
   }
-  // p = exp(x - m) / sum, of a row with m > -inf.
-  __device__ __forceinline__ void softmax(float m, float (&p)[C][V]) const {
+  // p = exp(x - m) / sum, and the sum: 0 where all is -inf (p means nothing then), NaN
+  // where a NaN is in the row, which max() passes over.
+  __device__ __forceinline__ float softmax(float m, float (&p)[C][V]) const {
+    if (m == -INFINITY) m = 0.f;
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < C; ++j)
@@ -78,11 +80,13 @@ struct Row {
         p[j][i] = __builtin_amdgcn_exp2f((x[j][i] - m) * 1.44269504088896341f);
         s += p[j][i];
       }
-    const float r = 1.f / group_sum<G>(s);
+    s = group_sum<G>(s);
+    const float r = 1.f / s;
 #pragma unroll
     for (int j = 0; j < C; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) p[j][i] *= r;
+    return s;
   }
 };
 
@@ -174,9 +178,8 @@ __global__ __launch_bounds__(kThreads) void balance_fwd_kernel(const T *__restri
     row.open(E, t);
     load(r + step, use_next);
     const float m = row.max();
-    const bool keep = use && m > -INFINITY;  // the same in all lanes of a group
     float p[C][V];
-    row.softmax(keep ? m : 0.f, p);
+    const bool keep = row.softmax(m, p) != 0.f && use;  // the same in all lanes of a group
 #pragma unroll
     for (int j = 0; j < C; ++j)
 #pragma unroll
@@ -283,9 +286,8 @@ __global__ __launch_bounds__(kBlock) void balance_bwd_kernel(const T *__restrict
     const uint8_t used = use;
     load(r + step);
     const float m = row.max();
-    const bool keep = used && m > -INFINITY;
     float p[C][V];
-    row.softmax(keep ? m : 0.f, p);
+    const bool keep = row.softmax(m, p) != 0.f && used;
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < C; ++j)

@@ -11,7 +11,7 @@ over the n positions that count:
 which is 1 for a balanced router and E / top_k at worst.  The counts are whole
 numbers without a gradient; the loss's flows through p.  Positions whose mask is
 False count nowhere, whatever their logits hold, and so do positions whose
-experts are all at -inf.
+experts are all at -inf.  A NaN in a position that counts makes the loss NaN.
 """
 
 from __future__ import annotations

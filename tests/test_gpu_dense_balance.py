@@ -78,6 +78,23 @@ def test_masks_and_excluded_experts(E, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E", [1, 7, 64, 300])
+def test_rows_of_nan_are_not_taken_for_excluded_ones(E, dtype):
+    announce(f"balance rows of NaN E={E} {dtype}")
+    x, _ = _logits(E, 200, E, dtype)
+    x[3] = -float("inf")
+    clean, counts = expert_balance(x.to(DEV), 1)
+    x[7] = -float("inf")
+    x[7, E - 1] = float("nan")
+    leaf = x.to(DEV).requires_grad_()
+    loss, bad = expert_balance(leaf, 1)
+    (d,) = torch.autograd.grad(loss, [leaf])
+    assert torch.isfinite(clean).item() and counts.sum().item() == 199
+    assert torch.isnan(loss).item() and bad.sum().item() == 198  # nothing is chosen of such a row
+    assert torch.isnan(d[7]).all() and torch.equal(d[3], torch.zeros_like(d[3]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_no_positions_and_all_masked(dtype):
     announce(f"balance empty {dtype}")
     for T in (0, 9):
