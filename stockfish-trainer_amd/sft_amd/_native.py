@@ -841,9 +841,38 @@ def _scratch(nbytes: int, device: torch.device):
     return buf, buf.data_ptr()
 
 
+def _like(what: str, t: torch.Tensor | None, shape: tuple, dtype: torch.dtype, device: torch.device,
+          dense: bool = True) -> None:
+    """Refuses a t (None: nothing to check) that a kernel would read or write out of range or as another type."""
+    if t is None:
+        return
+    _require(tuple(t.shape) == shape, f"{what} must be {list(shape)}, got {list(t.shape)}")
+    _require(t.dtype == dtype, f"{what} must be {dtype}, got {t.dtype}")
+    _require(not dense or t.is_contiguous(), f"{what} must be contiguous")
+    _require(t.device == device, f"{what} must be on {device}, got {t.device}")
+
+
+def _matrix(what: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, columns, type code) of a 2-D tensor on a GPU."""
+    _require(t.dim() == 2, f"{what} must have 2 dimensions, got {t.dim()}")
+    return *t.shape, type_code(t.dtype)
+
+
+def deriv_dtype(dtype: torch.dtype) -> torch.dtype:
+    """What act' of a layer of this type is kept as: binary32, or 16-bit fixed point."""
+    return torch.float32 if dtype == torch.float32 else torch.int16
+
+
 def linear_fwd(x, w, bias, residual, y, deriv, act: int) -> None:
     """y = residual + act(x w^T + bias) of 2-D tensors with dense rows; deriv (or None) gets act'."""
-    (M, K), N = x.shape, w.shape[0]
+    M, K, _ = _matrix("x", x)
+    N = _matrix("weight", w)[0]
+    _like("weight", w, (N, K), x.dtype, x.device, False)
+    _like("bias", bias, (N,), x.dtype, x.device)
+    _like("residual", residual, (M, N), x.dtype, x.device, False)
+    _like("y", y, (M, N), x.dtype, x.device, False)
+    _like("deriv", deriv, (M, N), deriv_dtype(x.dtype), x.device)
+    _on_gpu(x.device)
     code, dev = type_code(x.dtype), x.device
     n = ctypes.c_size_t(0)
     _check(lib().sft_linear_fwd_workspace_size(code, M, K, N, _copy_flag(x, w), ctypes.byref(n)),
@@ -856,7 +885,14 @@ def linear_fwd(x, w, bias, residual, y, deriv, act: int) -> None:
 
 def linear_bwd(dy, deriv, x, w, dx, dw, db, act: int) -> None:
     """dx, dw and db (each may be None) of linear_fwd's y from dy and its deriv."""
-    (M, K), N = x.shape, w.shape[0]
+    M, K, _ = _matrix("x", x)
+    N = _matrix("weight", w)[0]
+    _like("weight", w, (N, K), x.dtype, x.device, False)
+    _like("grad_y", dy, (M, N), x.dtype, x.device, False)
+    _like("deriv", deriv, (M, N), deriv_dtype(x.dtype), x.device)
+    for what, t, shape in (("dx", dx, (M, K)), ("dw", dw, (N, K)), ("db", db, (N,))):
+        _like(what, t, shape, x.dtype, x.device)
+    _on_gpu(x.device)
     code, dev = type_code(dy.dtype), dy.device
     n = ctypes.c_size_t(0)
     _check(lib().sft_linear_bwd_workspace_size(code, M, K, N, act, _copy_flag(dy, x, w), ctypes.byref(n)),
@@ -869,8 +905,13 @@ def linear_bwd(dy, deriv, x, w, dx, dw, db, act: int) -> None:
 
 def balance_fwd(logits, mask, top_k: int, loss, counts, kept) -> None:
     """loss (float32), counts (int64 [E]) and kept (int64) of the router's 2-D logits; mask bool [T] or None."""
-    T, E = logits.shape
-    code, dev = type_code(logits.dtype), logits.device
+    T, E, code = _matrix("logits", logits)
+    dev = logits.device
+    _like("mask", mask, (T,), torch.bool, dev)
+    _like("loss", loss, (), torch.float32, dev)
+    _like("counts", counts, (E,), torch.int64, dev)
+    _like("kept", kept, (), torch.int64, dev)
+    _on_gpu(dev)
     n = ctypes.c_size_t(0)
     _check(lib().sft_balance_fwd_workspace_size(code, T, E, ctypes.byref(n)), "sft_balance_fwd_workspace_size")
     keep, ws = _scratch(n.value, dev)
@@ -881,15 +922,30 @@ def balance_fwd(logits, mask, top_k: int, loss, counts, kept) -> None:
 
 def balance_bwd(logits, mask, top_k: int, counts, kept, grad_loss, grad_logits) -> None:
     """grad_logits (dense) of balance_fwd's loss times grad_loss (float32 on the device)."""
-    T, E = logits.shape
-    _call("sft_balance_bwd", logits.device, type_code(logits.dtype), logits.data_ptr(), _rows(logits), _at(mask), T, E,
+    T, E, code = _matrix("logits", logits)
+    dev = logits.device
+    _like("mask", mask, (T,), torch.bool, dev)
+    _like("counts", counts, (E,), torch.int64, dev)
+    _like("kept", kept, (), torch.int64, dev)
+    _like("grad_loss", grad_loss, (), torch.float32, dev)
+    _like("grad_logits", grad_logits, (T, E), logits.dtype, dev)
+    _on_gpu(dev)
+    _call("sft_balance_bwd", dev, code, logits.data_ptr(), _rows(logits), _at(mask), T, E,
           top_k, counts.data_ptr(), kept.data_ptr(), grad_loss.data_ptr(), grad_logits.data_ptr())
 
 
 def distill(student, teacher, indices, temperature: float, row_weight, loss, grad_student) -> None:
     """loss (float32 [R]) and grad_student (dense), each may be None, of 2-D logits and a teacher's dense top ones."""
-    R, V = student.shape
-    _call("sft_distill", student.device, type_code(student.dtype), student.data_ptr(), _rows(student),
+    R, V, code = _matrix("student logits", student)
+    k, dev = _matrix("teacher logits", teacher)[1], student.device
+    _like("teacher logits", teacher, (R, k), teacher.dtype, dev)
+    _require(indices.dtype in (torch.int32, torch.int64), f"indices must be int32 or int64, got {indices.dtype}")
+    _like("indices", indices, (R, k), indices.dtype, dev)
+    _like("row_weight", row_weight, (R,), torch.float32, dev)
+    _like("loss", loss, (R,), torch.float32, dev)
+    _like("grad_student", grad_student, (R, V), student.dtype, dev)
+    _on_gpu(dev)
+    _call("sft_distill", dev, code, student.data_ptr(), _rows(student),
           type_code(teacher.dtype), teacher.data_ptr(), indices.data_ptr(), indices.element_size(), R, V,
           teacher.shape[1], temperature, _at(row_weight), _at(loss), _at(grad_student))
 

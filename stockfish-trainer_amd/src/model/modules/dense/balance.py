@@ -51,5 +51,7 @@ def expert_balance(logits: Tensor, top_k: int = 1, mask: Tensor | None = None) -
     positions that count (None: all)."""
     if not torch.compiler.is_compiling():
         return _native.dense_binding().balance(logits, top_k, mask)
+    if mask is not None and mask.shape != logits.shape[:-1]:
+        raise ValueError("mask must be logits' shape without the last")
     mask = None if mask is None else mask.reshape(-1).contiguous()
     return ExpertBalanceFunction.apply(logits.reshape(-1, logits.shape[-1]), mask, top_k)

@@ -69,6 +69,8 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, residual
         return _native.dense_binding().linear(x, weight, bias, residual, act)
     N, K = weight.shape
     lead = x.shape[:-1]
+    if x.shape[-1] != K or (residual is not None and residual.shape != (*lead, N)):
+        raise ValueError("x must be [..., K] and residual [..., N]")
     x = x.reshape(-1, K)
     residual = None if residual is None else residual.reshape(-1, N)
     return FusedLinearFunction.apply(x, weight, bias, residual, act).view(*lead, N)

@@ -14,10 +14,6 @@ from torch import Tensor
 from sft_amd import _native
 
 
-def _deriv_dtype(dtype: torch.dtype) -> torch.dtype:
-    return torch.float32 if dtype == torch.float32 else torch.int16
-
-
 # ---- FusedLinearFunction ----
 @torch.library.custom_op("sft::linear_fwd", mutates_args=(), device_types="cuda")
 def linear_fwd(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor | None, act: int,
@@ -26,7 +22,7 @@ def linear_fwd(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor 
     M, N = x.shape[0], weight.shape[0]
     y = torch.empty(M, N, dtype=x.dtype, device=x.device)
     kept = keep and act != _native.SFT_ACT_NONE
-    deriv = torch.empty((M, N) if kept else (0,), dtype=_deriv_dtype(x.dtype), device=x.device)
+    deriv = torch.empty((M, N) if kept else (0,), dtype=_native.deriv_dtype(x.dtype), device=x.device)
     _native.linear_fwd(x, weight, bias, residual, y, deriv if kept else None, act)
     return y, deriv
 
@@ -35,7 +31,7 @@ def linear_fwd(x: Tensor, weight: Tensor, bias: Tensor | None, residual: Tensor 
 def _(x, weight, bias, residual, act, keep):
     shape = (x.shape[0], weight.shape[0])
     kept = keep and act != _native.SFT_ACT_NONE
-    return x.new_empty(shape), x.new_empty(shape if kept else (0,), dtype=_deriv_dtype(x.dtype))
+    return x.new_empty(shape), x.new_empty(shape if kept else (0,), dtype=_native.deriv_dtype(x.dtype))
 
 
 @torch.library.custom_op("sft::linear_bwd", mutates_args=(), device_types="cuda")

@@ -144,6 +144,53 @@ def test_distill_refuses(at, value, needle):
     assert rc == -1 and "neither" in why
 
 
+SHORTER = lambda t: t[:-1].contiguous()
+NARROWER = lambda t: t[..., :-1].contiguous()
+
+
+@pytest.mark.parametrize("call,at,wrong,needle", [
+    ("linear_fwd", "w", NARROWER, "weight must be"), ("linear_fwd", "w", torch.Tensor.float, "weight must be"),
+    ("linear_fwd", "bias", SHORTER, "bias must be"), ("linear_fwd", "bias", torch.Tensor.float, "bias must be"),
+    ("linear_fwd", "residual", SHORTER, "residual must be"), ("linear_fwd", "residual", NARROWER, "residual must be"),
+    ("linear_fwd", "y", SHORTER, "y must be"), ("linear_fwd", "deriv", torch.Tensor.half, "deriv must be"),
+    ("linear_fwd", "x", torch.Tensor.double, "dtype"), ("linear_fwd", "x", torch.Tensor.flatten, "2 dimensions"),
+    ("linear_fwd", "y", torch.Tensor.clone, "on a GPU"),
+    ("linear_bwd", "dy", SHORTER, "grad_y must be"), ("linear_bwd", "dy", torch.Tensor.float, "grad_y must be"),
+    ("linear_bwd", "deriv", SHORTER, "deriv must be"), ("linear_bwd", "dw", SHORTER, "dw must be"),
+    ("linear_bwd", "db", SHORTER, "db must be"), ("linear_bwd", "dx", NARROWER, "dx must be"),
+    ("linear_bwd", "dy", torch.Tensor.clone, "on a GPU"),
+    ("balance_fwd", "mask", SHORTER, "mask must be"), ("balance_fwd", "mask", torch.Tensor.float, "mask must be"),
+    ("balance_fwd", "counts", SHORTER, "counts must be"), ("balance_fwd", "loss", torch.Tensor.double, "loss must be"),
+    ("balance_fwd", "mask", torch.Tensor.clone, "on a GPU"),
+    ("balance_bwd", "mask", SHORTER, "mask must be"), ("balance_bwd", "grad_loss", torch.Tensor.half, "grad_loss must"),
+    ("balance_bwd", "grad_logits", NARROWER, "grad_logits must"), ("balance_bwd", "mask", torch.Tensor.clone, "on a GPU"),
+    ("distill", "teacher", SHORTER, "teacher logits must"), ("distill", "teacher", torch.Tensor.double, "dtype"),
+    ("distill", "indices", NARROWER, "indices must"), ("distill", "indices", torch.Tensor.short, "indices must"),
+    ("distill", "row_weight", SHORTER, "row_weight must"), ("distill", "row_weight", torch.Tensor.half, "row_weight must"),
+    ("distill", "loss", SHORTER, "loss must"), ("distill", "grad_student", torch.Tensor.float, "grad_student must"),
+    ("distill", "loss", torch.Tensor.clone, "on a GPU")])
+def test_calls_refuse_tensors_that_do_not_fit(call, at, wrong, needle):
+    """What traced programs reach: a tensor too short would be read past its end."""
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    n = lambda *s: torch.zeros(*s, dtype=torch.int64)
+    good = {
+        "linear_fwd": {"x": b(9, 5), "w": b(7, 5), "bias": b(7), "residual": b(9, 7), "y": b(9, 7),
+                       "deriv": torch.zeros(9, 7, dtype=torch.int16), "act": 5},
+        "linear_bwd": {"dy": b(9, 7), "deriv": torch.zeros(9, 7, dtype=torch.int16), "x": b(9, 5), "w": b(7, 5),
+                       "dx": b(9, 5), "dw": b(7, 5), "db": b(7), "act": 5},
+        "balance_fwd": {"logits": b(9, 6), "mask": torch.zeros(9, dtype=torch.bool), "top_k": 2,
+                        "loss": torch.zeros(()), "counts": n(6), "kept": n(())},
+        "balance_bwd": {"logits": b(9, 6), "mask": torch.zeros(9, dtype=torch.bool), "top_k": 2, "counts": n(6),
+                        "kept": n(()), "grad_loss": torch.zeros(()), "grad_logits": b(9, 6)},
+        "distill": {"student": b(9, 30), "teacher": torch.zeros(9, 2), "indices": n(9, 2), "temperature": 1.0,
+                    "row_weight": torch.zeros(9), "loss": torch.zeros(9), "grad_student": b(9, 30)},
+    }[call]
+    args = dict(good)
+    args[at] = wrong(args[at])
+    with pytest.raises(ValueError, match=needle):
+        getattr(_native, call)(*args.values())
+
+
 def test_custom_op_shapes():
     with FakeTensorMode():
         e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="cuda")
